@@ -29,6 +29,11 @@ workspace), ``validate`` returns a reason string or None.
 descriptor-ready weight layout) and :func:`fp8_decode_gemm` is a one-call
 torch entry point.  Everything runs through the CUDA library; when it is
 missing, importing the launch functions raises.
+
+The operators between two products of a decode layer -- block tables
+(:func:`build_block_tables`), rotary positions (:func:`rotary`,
+:func:`rotary_append`) and attention over a paged cache
+(:func:`paged_attention`) -- are in :mod:`decode_opt_b200.attention`.
 """
 
 from __future__ import annotations
@@ -51,7 +56,23 @@ __all__ = [
     "LAYOUT_RAW", "LAYOUT_PACKED", "LAYOUT_PACKED_SWIZZLED", "FLAG_INJECT_TIMEOUT", "FLAG_INDEPENDENT_INPUTS",
     "FLAG_SWAP_AB",
     "ERR_INJECTED_TIMEOUT", "STATUS_OK", "m_tile_for", "flush_l2", "GRID_CLUSTER", "copy_from_host",
+    "StepTables", "build_block_tables", "rope_table", "rotary", "rotary_append", "paged_attention",
+    "attention_workspace",
 ]
+
+# The attention operators (attention.py): loaded on first use, as that module
+# imports torch and this one does not.
+_ATTENTION = frozenset(("StepTables", "build_block_tables", "rope_table", "rotary", "rotary_append",
+                        "paged_attention", "attention_workspace"))
+
+
+def __getattr__(name):
+    if name in _ATTENTION:
+        from . import attention
+        globals()[name] = value = getattr(attention, name)
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
 
 CUDA_SUCCESS = 0
 CUDA_ERROR_INVALID_VALUE = 1

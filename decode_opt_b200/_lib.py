@@ -13,7 +13,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdecode_gemm_b200.so")
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 LAYOUT_RAW = 0
 LAYOUT_PACKED = 1
@@ -38,7 +38,17 @@ EXPORTED_SYMBOLS = (
     "dg_launch_gather", "dg_gather_wait", "dg_ipc_export", "dg_ipc_import", "dg_ipc_release",
     "dg_quantize_act", "dg_max_active_clusters", "dg_launch_quantized", "dg_launch_gather_lines",
     "dg_host_device_pointer", "dg_copy_from_host",
+    # include/decode_attention_b200.h
+    "dg_build_block_tables", "dg_rotary", "dg_paged_attention", "dg_attention_workspace_bytes",
 )
+
+# include/decode_attention_b200.h
+TYPE_BF16, TYPE_FP16, TYPE_FP32, TYPE_E4M3 = 0, 1, 2, 3
+PAIR_HALF, PAIR_ADJACENT = 0, 1
+MAX_ROT = 512                   # DG_MAX_ROT
+ERR_LENGTH, ERR_POOL, ERR_TABLE_WIDTH, ERR_TOKENS = 0xA1, 0xA2, 0xA3, 0xA4
+ERR_POSITION, ERR_SLOT = 0xB1, 0xB2
+ERR_PAGE, ERR_SEQ_LEN = 0xC1, 0xC2
 
 
 class DgConfig(ctypes.Structure):
@@ -125,6 +135,109 @@ class DgGatherLines(ctypes.Structure):
     ]
 
 
+class DgBlockTables(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("table_width", ctypes.c_int),
+        ("num_tokens", ctypes.c_int),
+        ("free_count", ctypes.c_int),
+        ("table_stride", ctypes.c_longlong),
+        ("context_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p),
+        ("free_pages", ctypes.c_void_p),
+        ("cursor_in", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start", ctypes.c_void_p),
+        ("slots", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("requests", ctypes.c_void_p),
+        ("cursor_out", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+    ]
+
+
+_Stride2 = ctypes.c_longlong * 2
+_Stride3 = ctypes.c_longlong * 3
+
+
+class DgRotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("tokens", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("rot", ctypes.c_int),
+        ("type", ctypes.c_int),
+        ("cache_type", ctypes.c_int),
+        ("pairing", ctypes.c_int),
+        ("inverse", ctypes.c_int),
+        ("position_64", ctypes.c_int),
+        ("max_position", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("k_out", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("q_stride", _Stride2),
+        ("k_stride", _Stride2),
+        ("v_stride", _Stride2),
+        ("q_out_stride", _Stride2),
+        ("k_out_stride", _Stride2),
+        ("k_cache_stride", _Stride3),
+        ("v_cache_stride", _Stride3),
+        ("positions", ctypes.c_void_p),
+        ("position_stride", ctypes.c_longlong),
+        ("slots", ctypes.c_void_p),
+        ("cos_sin", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("axis_of", ctypes.c_uint * (MAX_ROT // 32)),
+    ]
+
+
+class DgAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int),
+        ("heads", ctypes.c_int),
+        ("kv_heads", ctypes.c_int),
+        ("head_dim", ctypes.c_int),
+        ("page_size", ctypes.c_int),
+        ("num_pages", ctypes.c_int),
+        ("table_width", ctypes.c_int),
+        ("type", ctypes.c_int),
+        ("cache_type", ctypes.c_int),
+        ("window", ctypes.c_int),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+        ("q", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("q_stride", _Stride2),
+        ("k_cache_stride", _Stride3),
+        ("v_cache_stride", _Stride3),
+        ("block_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_longlong),
+        ("seq_lens", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("out", ctypes.c_void_p),
+        ("out_stride", _Stride2),
+        ("lse", ctypes.c_void_p),
+        ("q_out", ctypes.c_void_p),
+        ("q_scales", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_ulonglong),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 TensorMap = ctypes.c_uint8 * 128
 IpcHandle = ctypes.c_uint8 * 64
 
@@ -183,6 +296,10 @@ def lib():
     L.dg_ipc_release.argtypes = [ctypes.c_void_p]
     L.dg_probe_mma.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
+    L.dg_build_block_tables.argtypes = [ctypes.POINTER(DgBlockTables), ctypes.c_void_p, ctypes.c_int]
+    L.dg_rotary.argtypes = [ctypes.POINTER(DgRotaryArgs), ctypes.c_void_p, ctypes.c_int]
+    L.dg_paged_attention.argtypes = [ctypes.POINTER(DgAttentionArgs), ctypes.c_void_p, ctypes.c_int]
+    L.dg_attention_workspace_bytes.restype = ctypes.c_ulonglong
     if L.dg_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH}: ABI version {L.dg_abi_version()} != {ABI_VERSION}")
     _LIB = L

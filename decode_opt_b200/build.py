@@ -1,8 +1,10 @@
 """Build recipe for the in-tree sm_100a libraries.
 
-``python -m decode_opt_b200.build`` compiles ``csrc/dg_capi.cu`` into
-``decode_opt_b200/libdecode_gemm_b200.so`` for ``sm_100a`` only.  The library
-links the CUDA runtime statically and resolves ``cuTensorMapEncodeTiled``
+``python -m decode_opt_b200.build`` compiles the library's sources in ``csrc/``
+(``SOURCES``: the GEMM and its C ABI, probes, quantiser, and the attention
+operators) into ``decode_opt_b200/libdecode_gemm_b200.so`` for ``sm_100a``
+only, the files side by side.  The library links
+the CUDA runtime statically and resolves ``cuTensorMapEncodeTiled``
 through the runtime's driver entry-point query, so it loads on hosts without a
 GPU (the CPU test suite checks its exported symbols there).
 
@@ -34,7 +36,7 @@ CUBLASLT_SRC = os.path.join(CSRC, "dg_cublaslt_fp8.cu")
 CUBLASLT_BIN = os.path.join(HERE, "dg_cublaslt_fp8")
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
-SOURCES = ("dg_capi.cu", "dg_probe.cu", "dg_quant.cu")
+SOURCES = ("dg_capi.cu", "dg_probe.cu", "dg_quant.cu", "dg_block_tables.cu", "dg_rotary.cu", "dg_attention.cu")
 
 
 def nvcc() -> str:
@@ -98,7 +100,7 @@ def build_library(verbose: bool = False, ptxas_verbose: bool = False, force: boo
     if not force and not needs_build():
         return LIB_PATH
     cmd = [nvcc(), "-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS,
-           "-Xcompiler", "-fPIC", "-shared", "-cudart", "static",
+           "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "--threads", "0",
            "-I", CSRC, "-I", INCLUDE,
            *[os.path.join(CSRC, f) for f in SOURCES], "-o", LIB_PATH + ".tmp"]
     if ptxas_verbose:

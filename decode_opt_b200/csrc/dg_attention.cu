@@ -1,0 +1,939 @@
+// SPDX-License-Identifier: MIT
+//
+// dg_attention.cu -- attention of one new token per request over a paged
+// key-value cache (include/decode_attention_b200.h gives the definition).
+//
+// Bound: the live tokens' keys and values are read once per kv head, 2 * D
+// values a token, against 4 * D operations a token and query head: with up to
+// about 100 query heads on a kv head that is HBM traffic, so everything here
+// serves to keep enough 16-byte copies in flight on every SM.
+//
+// Split.  The work is cut into tiles of TOK tokens of one (request, kv head,
+// group of ROWS query heads) "item"; all tiles of all items stand in one
+// line, and CTA c of G takes tiles [W c / G, W (c+1) / G) of it -- equal shares
+// whatever the lengths are, one CTA an SM.  The line is laid out on the
+// device from seq_lens (one scan of the batch per CTA), so that the host
+// needs no lengths.  A CTA therefore works on a run of items: the first and
+// the last may be shared with its neighbours, those between are its own.
+// Within an item's share the CTA's warps take tiles in turn, each with its
+// own ring of TOK-token stages filled by its own cp.async copies: no barrier
+// in the loop, and the ring runs on across items, so that the end of one
+// does not drain it.  16-byte copies with the row's address from the page
+// table (one table entry per token and lane, fetched a tile ahead) take any
+// page size and strides; tokens that are not live are zero-filled and masked.
+//
+// Products: mma.sync m16n8k16, the query heads as its 16 rows.  At 16 rows
+// the tensor pipe is far from its limit at HBM speed (43 bytes a ns and SM
+// are 1/6 of what it takes), so the roomier tcgen05 shapes (64 or 128 rows)
+// would only multiply zeros.  Scores stay in registers: the accumulator
+// layout of S = Q K^T is the operand layout of P V.  P enters as two terms,
+// hi = p cut to 16 bits and lo = round(p - hi), so that its rounding (2^-8 in
+// bf16) does not show in the result: with up to 8 query heads a kv head
+// (ROWS = 8) the lo terms fill the 8 rows that would be empty, at no cost;
+// with more (ROWS = 16) they are a second product.  Cut towards zero and with
+// lo kept above 0, both terms have the sign of p, so that an infinite value
+// stays infinite (0 times it would be NaN).
+//
+// e4m3 caches are widened to fp16 (exact) on the way into the product.  Both
+// products are indifferent to the order of their inner index, and the columns
+// of the second to a permutation, so that fragments are read as 16 and 8
+// consecutive bytes a lane: no 8-bit transposition.  q is scaled by a power
+// of two per head to fit fp16's range, exactly undone in fp32.
+//
+// Join.  The warps' (m, l, o) are joined in shared memory, 32 columns at a
+// time, in warp order.  A share of an item goes to the workspace; the last
+// of the item's CTAs to arrive (a ticket) joins the shares in CTA order.
+// No CTA waits for another.
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <cstdint>
+
+#include "decode_attention_b200.h"
+#include "decode_gemm_b200.h"
+#include "sm100.cuh"
+#include "warp_mma.cuh"
+
+namespace {
+
+using dg::warp::Bf16;
+using dg::warp::Fp16;
+
+constexpr int kMaxCtas = 160;            // CTAs of a launch: one an SM (148)
+constexpr int kMaxRows = 16;             // query heads an item
+constexpr int kMaxDim = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFp8Max = 448.0f;        // of the output's quantisation, as dg_quantize_act
+constexpr float kQuantEps = 1.0e-4f;
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Workspace: tickets, then (m, l) per share and row, then the shares.
+constexpr size_t kTicketBytes = 1024;    // kMaxCtas ints
+constexpr size_t kShares = 2 * kMaxCtas; // a CTA's first and last item
+constexpr size_t kWorkspaceBytes =
+    kTicketBytes + kShares * kMaxRows * sizeof(float2) + kShares * kMaxRows * kMaxDim * sizeof(float);
+static_assert(kMaxCtas * sizeof(int) <= kTicketBytes, "tickets");
+
+struct Params {
+  dg_attention_args a;
+  int group;               // query heads a kv head
+  int groups;              // items a kv head: ceil(group / ROWS)
+  int page_shift;          // log2(page_size), -1 if it is no power of two
+  int* tickets;
+  float2* share_ml;        // [share][kMaxRows]
+  float* share_o;          // [share][kMaxRows][kMaxDim]
+};
+
+// Compile-time shape: MM the 16-bit type of the products, E4M3 the cache, DP
+// the head dimension padded to 64 / 128 / 256, ROWS the query heads an item.
+template <typename MM_, bool E4M3_, int DP_, int ROWS_>
+struct Shape {
+  using MM = MM_;
+  static constexpr bool kE4m3 = E4M3_;
+  static constexpr int DP = DP_, ROWS = ROWS_;
+  static constexpr int ES = E4M3_ ? 1 : 2;
+  static constexpr int NW = DP_ == 256 ? 4 : 8;                  // warps
+  static constexpr int TOK = E4M3_ || DP_ == 64 ? 32 : 16;       // tokens a stage
+  static constexpr int STAGES = 3;
+  static constexpr int PITCH = DP_ * ES;                         // bytes a row
+  static constexpr int KV_BYTES = TOK * PITCH;                   // a stage's keys; its values follow
+  static constexpr int STAGE = 2 * KV_BYTES;
+  static constexpr int RING = NW * STAGES * STAGE;
+  static constexpr int JOIN_ROW = 40;                            // 32 columns, padded against bank conflicts
+  static constexpr int JOIN_BUFS = ROWS_ == 8 ? 2 : 1;
+  static constexpr int JOIN = NW * ROWS_ * JOIN_ROW;             // floats a buffer
+  static constexpr int NT = TOK / 8;                             // score tiles of 8 tokens
+  static constexpr int KS = DP_ / 16;                            // inner steps of Q K^T
+  static constexpr int OT = DP_ / 8;                             // output tiles of 8 columns
+  static constexpr int CHUNKS = DP_ / 32;                        // of the joins
+  static constexpr int RPT = ROWS_ / NW;                         // rows a warp finishes
+  // 2^kBias is the probability of the maximum: fp16's subnormals start at
+  // 2^-14, so its probabilities are lifted out of them.
+  static constexpr float kBias = sizeof(MM_) != 0 && __is_same(MM_, Fp16) ? 10.0f : 0.0f;
+  static constexpr size_t SMEM = RING + sizeof(float) * (JOIN_BUFS * JOIN + 2 * NW * ROWS_) +
+                                 sizeof(uint32_t) * NW * STAGES;
+  static_assert(ROWS_ % NW == 0 && SMEM <= 227 * 1024 - 1024, "shared memory");
+  static_assert(kMaxCtas * ROWS_ <= JOIN_BUFS * JOIN, "join factors fit the join buffers");
+
+  // Output column of position `n` of output tile `t` (see the e4m3 fragments).
+  static __device__ __forceinline__ int column(int t, int n) {
+    return E4M3_ ? (t >> 3) * 64 + n * 8 + (t & 7) : t * 8 + n;
+  }
+  // Where row `r` keeps its 16-byte chunk `c`: the eight chunks that one phase
+  // of the fragment loads reads fall into different banks.  16-bit: one chunk
+  // of 8 consecutive rows.  e4m3: 4 chunks of rows (2i, 2i + 1) for keys, 2
+  // chunks of rows 0, 2, 4, 6 (or 1, 3, 5, 7) for values.
+  static __device__ __forceinline__ int swizzled(int r, int c) {
+    return E4M3_ ? c ^ ((r & 6) ^ ((r & 1) << 2)) : c ^ (r & 7);
+  }
+};
+
+__device__ __forceinline__ void report(int* status, int code) {
+  if (status != nullptr) atomicCAS(status, 0, code);
+}
+
+// A request's live tokens as tiles.
+struct Live {
+  int lo, len;    // live tokens [lo, len)
+  int first;      // first tile
+  int tiles;      // tiles, 0 if nothing is live
+};
+
+template <int TOK>
+__device__ __forceinline__ Live live_of(const dg_attention_args& a, int b, bool tell) {
+  Live v;
+  int len = a.seq_lens[b];
+  const long long most = static_cast<long long>(a.table_width) * a.page_size;
+  if (len < 0 || len > most) {
+    if (tell) report(a.status, DG_ERR_SEQ_LEN);
+    len = len < 0 ? 0 : static_cast<int>(most);
+  }
+  v.len = len;
+  v.lo = a.window > 0 && len > a.window ? len - a.window : 0;
+  v.first = v.lo / TOK;
+  v.tiles = len > 0 ? (len - 1) / TOK + 1 - v.first : 0;
+  return v;
+}
+
+// A place in a CTA's run of tiles: one item's share.
+template <int TOK>
+struct Cursor {
+  long long g, g1;       // the share's first tile in the line, end of the CTA's run
+  long long item_g0;     // the item's first tile in the line
+  int b, item;           // request, item of the request
+  int t0, count;         // the share: tiles [t0, t0 + count) of the item
+  Live live;
+
+  __device__ __forceinline__ void settle() {
+    count = static_cast<int>(min(static_cast<long long>(live.tiles - t0), g1 - g));
+  }
+  __device__ __forceinline__ void start(const dg_attention_args& a, int request, long long base, long long from,
+                                        long long to) {
+    b = request;
+    g = from;
+    g1 = to;
+    live = live_of<TOK>(a, b, false);
+    const long long off = from - base;
+    item = static_cast<int>(off / live.tiles);
+    t0 = static_cast<int>(off - static_cast<long long>(item) * live.tiles);
+    item_g0 = from - t0;
+    settle();
+  }
+  // To the next share; false at the end of the run.
+  __device__ __forceinline__ bool advance(const dg_attention_args& a, int items) {
+    g += count;
+    if (g >= g1) return false;
+    if (++item == items) {
+      item = 0;
+      do {
+        ++b;             // g < g1 <= W: a later request has tiles
+        live = live_of<TOK>(a, b, false);
+      } while (live.tiles == 0);
+    }
+    item_g0 = g;
+    t0 = 0;
+    settle();
+    return true;
+  }
+};
+
+// One warp's copies: tile after tile of the CTA's run, ahead of the products.
+template <typename S>
+struct Loader {
+  Cursor<S::TOK> at;
+  int tile;              // of the share: warp, warp + NW, ...
+  bool more;             // a tile is pending
+  // The pending tile: this lane's token.
+  int page, offset, head;
+  bool ok;
+
+  __device__ __forceinline__ void look_up(const Params& p, int lane) {
+    const int tok = (at.live.first + at.t0 + tile) * S::TOK + lane;
+    ok = lane < S::TOK && tok >= at.live.lo && tok < at.live.len;
+    page = -1;
+    offset = 0;
+    head = p.groups == 1 ? at.item : at.item / p.groups;
+    if (ok) {
+      const unsigned t = static_cast<unsigned>(tok);
+      unsigned column;
+      if (p.page_shift >= 0) {
+        column = t >> p.page_shift;
+        offset = static_cast<int>(t & ((1u << p.page_shift) - 1u));
+      } else {
+        column = t / static_cast<unsigned>(p.a.page_size);
+        offset = static_cast<int>(t - column * static_cast<unsigned>(p.a.page_size));
+      }
+      page = __ldg(p.a.block_table + at.b * p.a.table_stride + column);
+    }
+  }
+  // Moves to the warp's next tile, through the shares that have none for it.
+  __device__ __forceinline__ void prepare(const Params& p, int warp, int lane, int items) {
+    if (!more) return;
+    while (tile >= at.count) {
+      if (!at.advance(p.a, items)) {
+        more = false;
+        return;
+      }
+      tile = warp;
+    }
+    look_up(p, lane);
+    tile += S::NW;
+  }
+  // Copies the pending tile into a stage.
+  __device__ __forceinline__ void issue(const Params& p, uint32_t stage, uint32_t* mask, int lane) const {
+    if (!more) return;
+    const dg_attention_args& a = p.a;
+    bool good = ok;
+    if (ok && (page < 0 || page >= a.num_pages)) {
+      report(a.status, DG_ERR_PAGE);
+      good = false;
+    }
+    const uint32_t live = __ballot_sync(0xffffffffu, good);
+    if (lane == 0) *mask = live;
+    long long k_at = 0, v_at = 0;
+    if (good) {
+      k_at = page * a.k_cache_stride[0] + offset * a.k_cache_stride[1] + head * a.k_cache_stride[2];
+      v_at = page * a.v_cache_stride[0] + offset * a.v_cache_stride[1] + head * a.v_cache_stride[2];
+    }
+    constexpr int CH = S::DP * S::ES / 16;      // chunks a row
+    constexpr int RPI = 32 / CH;                // rows an instruction
+    const int chunk = lane % CH;
+    const bool wanted = chunk * 16 < a.head_dim * S::ES;
+#pragma unroll
+    for (int i = 0; i < S::TOK / RPI; ++i) {
+      const int r = i * RPI + lane / CH;
+      const long long kr = __shfl_sync(0xffffffffu, k_at, r);
+      const long long vr = __shfl_sync(0xffffffffu, v_at, r);
+      const uint32_t bytes = (live >> r) & 1u ? 16u : 0u;
+      const uint32_t dst = stage + r * S::PITCH + S::swizzled(r, chunk) * 16;
+      if (wanted) {
+        dg::warp::cp_async16(dst, static_cast<const char*>(a.k_cache) + kr * S::ES + (bytes ? chunk * 16 : 0), bytes);
+        dg::warp::cp_async16(dst + S::KV_BYTES,
+                             static_cast<const char*>(a.v_cache) + vr * S::ES + (bytes ? chunk * 16 : 0), bytes);
+      }
+    }
+  }
+};
+
+// A pair of q's values as floats.
+__device__ __forceinline__ float2 unpack_q(uint32_t v, int type) {
+  return type == DG_TYPE_BF16 ? Bf16::unpack(v) : Fp16::unpack(v);
+}
+
+// One warp's state for one item.
+template <typename S>
+struct Warp {
+  static constexpr int R = S::ROWS == 8 ? 1 : 2;     // rows a lane: lane / 4 (and + 8)
+  uint32_t q[S::KS][2 * R];                          // [step][first half's rows, second half's rows]
+  float o[S::OT][4];
+  float m[R], l[R];
+  float factor[R];                                   // score -> exponent of 2 (or -> argument of tanh)
+
+  __device__ __forceinline__ void begin(const Params& p, int b, int item, int lane) {
+    const dg_attention_args& a = p.a;
+    const int head = p.groups == 1 ? item : item / p.groups;
+    const int part = item - head * p.groups;
+    const int quad = lane & 3;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = part * S::ROWS + (lane >> 2) + 8 * r;
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] +
+                            (static_cast<long long>(head) * p.group + row) * a.q_stride[1];
+      const bool real = row < p.group;
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ++ks) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          // Inner index of the two values: as ldmatrix deals 16-bit keys, or
+          // 4 consecutive ones of the lane's 16 bytes of e4m3 keys.
+          const int d = S::kE4m3 ? (ks >> 2) * 64 + quad * 16 + (ks & 3) * 4 + h * 2 : ks * 16 + quad * 2 + h * 8;
+          q[ks][h * R + r] = real && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+        }
+      }
+      float f = a.scale;
+      if constexpr (S::kE4m3) {
+        float top = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 v = unpack_q(q[ks][h * R + r], a.type);
+            top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^-e and 2^e of top's exponent e; none for 0, subnormals, infinity.
+        const uint32_t e = __float_as_uint(top) >> 23;
+        const bool scaled = e > 0 && e < 254;
+        const float down = scaled ? __uint_as_float((254u - e) << 23) : 1.0f;
+        const float up = scaled ? __uint_as_float(e << 23) : 1.0f;
+#pragma unroll
+        for (int ks = 0; ks < S::KS; ++ks)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 v = unpack_q(q[ks][h * R + r], a.type);
+            q[ks][h * R + r] = Fp16::pack(v.x * down, v.y * down);
+          }
+        f *= up;
+        if (a.k_scale != nullptr) f *= a.k_scale[head];
+      }
+      factor[r] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
+      m[r] = kNegInf;
+      l[r] = 0.0f;
+    }
+#pragma unroll
+    for (int t = 0; t < S::OT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[t][i] = 0.0f;
+  }
+
+  __device__ __forceinline__ void a_of(int ks, uint32_t (&x)[4]) const {
+    if constexpr (R == 1) {
+      x[0] = q[ks][0];
+      x[1] = 0u;
+      x[2] = q[ks][1];
+      x[3] = 0u;
+    } else {
+      x[0] = q[ks][0];
+      x[1] = q[ks][1];
+      x[2] = q[ks][2];
+      x[3] = q[ks][3];
+    }
+  }
+
+  // One stage: TOK tokens, of which `live` are to be seen.
+  __device__ __forceinline__ void step(const Params& p, uint32_t keys, uint32_t live, int lane) {
+    const uint32_t values = keys + S::KV_BYTES;
+    const int g = lane >> 2, quad = lane & 3;
+    float s[S::NT][4];
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[t][i] = 0.0f;
+
+    if constexpr (!S::kE4m3) {
+      // Matrices: tokens 0-7 x (values 0-7, 8-15), tokens 8-15 x the same.
+      const int row = (lane & 7) + (lane >> 4) * 8, side = (lane >> 3) & 1;
+      const uint32_t at = keys + row * S::PITCH;
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ++ks) {
+        uint32_t x[4];
+        a_of(ks, x);
+#pragma unroll
+        for (int t = 0; t < S::NT; t += 2) {
+          uint32_t k[4];
+          dg::warp::ldmatrix_x4(k, at + t * 8 * S::PITCH + S::swizzled(lane, ks * 2 + side) * 16);
+          S::MM::mma(s[t], x, k[0], k[1]);
+          S::MM::mma(s[t + 1], x, k[2], k[3]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int blk = 0; blk < S::KS / 4; ++blk) {
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t) {
+          const int r = t * 8 + g;
+          const uint4 k = dg::warp::ld_shared_v4(keys + r * S::PITCH + S::swizzled(r, blk * 4 + quad) * 16);
+          const uint32_t w[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t x[4];
+            a_of(blk * 4 + i, x);
+            S::MM::mma(s[t], x, dg::warp::e4m3x2_to_f16x2(w[i]), dg::warp::e4m3x2_to_f16x2(w[i] >> 16));
+          }
+        }
+      }
+    }
+
+    // Exponents, masked; the running maximum and sum.
+    const bool capped = p.a.softcap > 0.0f;
+    const float cap = p.a.softcap * kLog2e;
+    const bool whole = live == (S::TOK == 32 ? 0xffffffffu : (1u << (S::TOK & 31)) - 1u);
+    float alpha[R];
+    bool moved = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float top = m[r];
+#pragma unroll
+      for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float x = s[t][2 * r + i] * factor[r];
+          if (capped) x = tanhf(x) * cap;
+          if (!whole && ((live >> (t * 8 + quad * 2 + i)) & 1u) == 0u) x = kNegInf;
+          s[t][2 * r + i] = x;
+          top = fmaxf(top, x);
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      moved = moved || top > m[r];
+      const float from = (top == kNegInf ? 0.0f : top) - S::kBias;
+      alpha[r] = dg::warp::exp2_approx((m[r] - top) == (m[r] - top) ? m[r] - top : kNegInf);
+      m[r] = top;
+      float sum = 0.0f;
+#pragma unroll
+      for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float e = dg::warp::exp2_approx(s[t][2 * r + i] - from);
+          s[t][2 * r + i] = e;
+          sum += e;
+        }
+      l[r] = l[r] * alpha[r] + sum;
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int t = 0; t < S::OT; ++t) {
+        o[t][0] *= alpha[0];
+        o[t][1] *= alpha[0];
+        o[t][2] *= alpha[R - 1];
+        o[t][3] *= alpha[R - 1];
+      }
+    }
+
+#pragma unroll
+    for (int kk = 0; kk < S::NT / 2; ++kk) {
+      // hi and lo of the probabilities of 16 tokens as the first operand.
+      uint32_t hi[2 * R], lo[2 * R];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float u = s[kk * 2 + h][2 * r], v = s[kk * 2 + h][2 * r + 1];
+          const uint32_t top = S::MM::cut(u, v);
+          const float2 back = S::MM::unpack(top);
+          hi[h * R + r] = top;
+          lo[h * R + r] = S::MM::pack(fmaxf(u - back.x, S::MM::kTiny), fmaxf(v - back.y, S::MM::kTiny));
+        }
+      uint32_t x[4], y[4];
+      if constexpr (R == 1) {
+        x[0] = hi[0];
+        x[1] = lo[0];          // rows 8-15: the low terms of rows 0-7
+        x[2] = hi[1];
+        x[3] = lo[1];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = hi[i];
+          y[i] = lo[i];
+        }
+      }
+      if constexpr (!S::kE4m3) {
+        const uint32_t at = values + (kk * 16 + (lane & 15)) * S::PITCH;
+#pragma unroll
+        for (int t = 0; t < S::OT; t += 2) {
+          uint32_t v[4];
+          dg::warp::ldmatrix_x4_trans(v, at + S::swizzled(lane, t + (lane >> 4)) * 16);
+          S::MM::mma(o[t], x, v[0], v[1]);
+          S::MM::mma(o[t + 1], x, v[2], v[3]);
+          if constexpr (R == 2) {
+            S::MM::mma(o[t], y, v[0], v[1]);
+            S::MM::mma(o[t + 1], y, v[2], v[3]);
+          }
+        }
+      } else {
+        // A lane holds 8 consecutive columns 64 j + 8 g of its tokens 2 quad,
+        // + 1, + 8, + 9: position g of the 8 output tiles of block j.
+#pragma unroll
+        for (int j = 0; j < S::DP / 64; ++j) {
+          uint2 v[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = kk * 16 + quad * 2 + (i & 1) + (i >> 1) * 8;
+            v[i] = dg::warp::ld_shared_v2(values + r * S::PITCH + S::swizzled(r, j * 4 + (g >> 1)) * 16 + (g & 1) * 8);
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            // Columns 2w and 2w + 1 of the 8, tokens paired.
+            const uint32_t sel = w & 1 ? 0x7362u : 0x5140u;
+            const uint32_t b0 = __byte_perm(w < 2 ? v[0].x : v[0].y, w < 2 ? v[1].x : v[1].y, sel);
+            const uint32_t b1 = __byte_perm(w < 2 ? v[2].x : v[2].y, w < 2 ? v[3].x : v[3].y, sel);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t f0 = dg::warp::e4m3x2_to_f16x2(b0 >> (16 * c));
+              const uint32_t f1 = dg::warp::e4m3x2_to_f16x2(b1 >> (16 * c));
+              S::MM::mma(o[j * 8 + w * 2 + c], x, f0, f1);
+              if constexpr (R == 2) S::MM::mma(o[j * 8 + w * 2 + c], y, f0, f1);
+            }
+          }
+        }
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ float max_ref(float a, float b) { return a < b ? b : a; }
+__device__ __forceinline__ float min_ref(float a, float b) { return b < a ? b : a; }
+
+__device__ __forceinline__ void store_out(const dg_attention_args& a, long long at, float v) {
+  if (a.type == DG_TYPE_BF16)
+    static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
+  else
+    static_cast<__half*>(a.out)[at] = __float2half_rn(v);
+}
+
+// A finished row: this lane's column of each 32-column chunk, unnormalised.
+template <typename S>
+__device__ __forceinline__ void finish_row(const Params& p, int b, int item, int row, const float (&v)[S::CHUNKS],
+                                           float m, float l, int lane) {
+  const dg_attention_args& a = p.a;
+  const int head = p.groups == 1 ? item : item / p.groups;
+  const int in_group = (item - head * p.groups) * S::ROWS + row;
+  if (in_group >= p.group) return;
+  const int h = head * p.group + in_group;
+  float norm = 1.0f / l;
+  if (S::kE4m3 && a.v_scale != nullptr) norm *= a.v_scale[head];
+  const long long at = b * a.out_stride[0] + h * a.out_stride[1];
+#pragma unroll
+  for (int c = 0; c < S::CHUNKS; ++c) {
+    const int d = S::column(c * 4 + (lane >> 3), lane & 7);
+    if (d < a.head_dim) store_out(a, at + d, v[c] * norm);
+  }
+  if (a.lse != nullptr && lane == 0)
+    a.lse[static_cast<long long>(b) * a.heads + h] = (m - S::kBias) * kLn2 + logf(l);
+  if constexpr (S::DP >= 128) {
+    if (a.q_out != nullptr) {
+      // 128 columns are 4 chunks; quantised as the rounded bf16 values.
+      const long long width = static_cast<long long>(a.heads) * a.head_dim;
+#pragma unroll
+      for (int blk = 0; blk < S::DP / 128; ++blk) {
+        if (blk * 128 >= a.head_dim) break;
+        float x[4], top = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          x[c] = __bfloat162float(__float2bfloat16_rn(v[blk * 4 + c] * norm));
+          top = max_ref(top, fabsf(x[c]));
+        }
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) top = max_ref(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float scale = max_ref(top, kQuantEps) / kFp8Max;
+        uint8_t* q = static_cast<uint8_t*>(a.q_out) + b * width + static_cast<long long>(h) * a.head_dim;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float y = min_ref(max_ref(x[c] / scale, -kFp8Max), kFp8Max);
+          q[S::column((blk * 4 + c) * 4 + (lane >> 3), lane & 7)] = __nv_fp8_e4m3(y).__x;
+        }
+        if (lane == 0) a.q_scales[(b * width + static_cast<long long>(h) * a.head_dim) / 128 + blk] = scale;
+      }
+    }
+  }
+}
+
+template <typename S>
+__global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_constant__ Params p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* join = reinterpret_cast<float*>(smem + S::RING);               // [JOIN_BUFS][NW][ROWS][JOIN_ROW]
+  float* warp_m = join + S::JOIN_BUFS * S::JOIN;                        // [NW][ROWS]
+  float* warp_l = warp_m + S::NW * S::ROWS;
+  uint32_t* masks = reinterpret_cast<uint32_t*>(warp_l + S::NW * S::ROWS);   // [NW][STAGES]
+  __shared__ long long scan_sum[S::NW];
+  __shared__ long long found_base;
+  __shared__ int found_request, is_last;
+
+  dg::sm100::griddep_launch_dependents();
+  dg::sm100::griddep_wait();
+
+  const dg_attention_args& a = p.a;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 31, warp = tid >> 5;
+  constexpr int kThreads = S::NW * 32;
+  const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
+  const int items = a.kv_heads * p.groups;
+
+  // Requests without live tokens, dealt over the CTAs.
+  for (int b = cta; b < a.batch; b += ctas) {
+    if (live_of<S::TOK>(a, b, tid == 0).tiles != 0) continue;
+    const long long width = static_cast<long long>(a.heads) * a.head_dim;
+    for (int h = warp; h < a.heads; h += S::NW)
+      for (int d = lane; d < a.head_dim; d += 32) {
+        store_out(a, b * a.out_stride[0] + h * a.out_stride[1] + d, 0.0f);
+        if (a.q_out != nullptr) static_cast<uint8_t*>(a.q_out)[b * width + h * a.head_dim + d] = 0;
+      }
+    for (int h = tid; h < a.heads && a.lse != nullptr; h += kThreads)
+      a.lse[static_cast<long long>(b) * a.heads + h] = kNegInf;
+    for (int i = tid; i < width / 128 && a.q_out != nullptr; i += kThreads)
+      a.q_scales[b * (width / 128) + i] = kQuantEps / kFp8Max;
+  }
+
+  // The line of tiles: its length, and the request where this CTA's run
+  // begins.
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += live_of<S::TOK>(a, b, false).tiles;
+  mine *= items;
+  long long scan = mine;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, scan, off);
+    if (lane >= off) scan += v;
+  }
+  if (lane == 31) scan_sum[warp] = scan;
+  // Columns past head_dim are never copied: zero in keys, values and q.
+  if (a.head_dim < S::DP)
+    for (int i = tid; i < S::RING / 16; i += kThreads) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  long long total = 0, before = scan - mine;
+#pragma unroll
+  for (int w = 0; w < S::NW; ++w) {
+    if (w < warp) before += scan_sum[w];
+    total += scan_sum[w];
+  }
+  // CTAs in use: at least one tile a warp.
+  const int used = static_cast<int>(min(static_cast<long long>(ctas), (total + S::NW - 1) / S::NW));
+  if (cta >= used) return;
+  const long long g0 = total * cta / used, g1 = total * (cta + 1) / used;
+  if (before <= g0 && g0 < before + mine) {
+    long long base = before;
+    int b = b0;
+    for (;; ++b) {
+      const long long n = static_cast<long long>(live_of<S::TOK>(a, b, false).tiles) * items;
+      if (g0 < base + n) break;
+      base += n;
+    }
+    found_request = b;
+    found_base = base;
+  }
+  __syncthreads();
+
+  Cursor<S::TOK> at;
+  at.start(a, found_request, found_base, g0, g1);
+  Loader<S> loader;
+  loader.at = at;
+  loader.tile = warp;
+  loader.more = true;
+  const uint32_t ring = dg::sm100::smem_addr(smem) + warp * (S::STAGES * S::STAGE);
+  uint32_t* mask = masks + warp * S::STAGES;
+  loader.prepare(p, warp, lane, items);
+#pragma unroll
+  for (int i = 0; i < S::STAGES - 1; ++i) {
+    loader.issue(p, ring + i * S::STAGE, mask + i, lane);
+    dg::warp::cp_async_commit();
+    loader.prepare(p, warp, lane, items);
+  }
+
+  Warp<S> w;
+  int stage = 0;
+  for (bool run = true; run; run = at.advance(a, items)) {
+    w.begin(p, at.b, at.item, lane);
+    for (int tile = warp; tile < at.count; tile += S::NW) {
+      dg::warp::cp_async_wait<S::STAGES - 2>();
+      __syncwarp();        // every lane's copies of this stage landed, every lane is done with the one before
+      const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
+      loader.issue(p, ring + ahead * S::STAGE, mask + ahead, lane);
+      dg::warp::cp_async_commit();
+      loader.prepare(p, warp, lane, items);
+      w.step(p, ring + stage * S::STAGE, mask[stage], lane);
+      stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+    }
+
+    // Join the warps.
+    const int g = lane >> 2, quad = lane & 3;
+#pragma unroll
+    for (int r = 0; r < Warp<S>::R; ++r) {
+      float l = w.l[r];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (quad == 0) {
+        warp_m[warp * S::ROWS + g + 8 * r] = w.m[r];
+        warp_l[warp * S::ROWS + g + 8 * r] = l;
+      }
+    }
+    __syncthreads();
+    float mine_by[Warp<S>::R];              // this warp's weight in the joined rows
+#pragma unroll
+    for (int r = 0; r < Warp<S>::R; ++r) {
+      float top = kNegInf;
+#pragma unroll
+      for (int v = 0; v < S::NW; ++v) top = fmaxf(top, warp_m[v * S::ROWS + g + 8 * r]);
+      mine_by[r] = w.m[r] == kNegInf ? 0.0f : dg::warp::exp2_approx(w.m[r] - top);
+    }
+    float row_m[S::RPT], row_l[S::RPT], sum[S::RPT][S::CHUNKS];
+#pragma unroll
+    for (int i = 0; i < S::RPT; ++i) {
+      const int row = warp + i * S::NW;
+      float top = kNegInf, l = 0.0f;
+#pragma unroll
+      for (int v = 0; v < S::NW; ++v) top = fmaxf(top, warp_m[v * S::ROWS + row]);
+#pragma unroll
+      for (int v = 0; v < S::NW; ++v) {
+        const float mv = warp_m[v * S::ROWS + row];
+        if (mv != kNegInf) l += warp_l[v * S::ROWS + row] * dg::warp::exp2_approx(mv - top);
+      }
+      row_m[i] = top;
+      row_l[i] = l;
+    }
+#pragma unroll
+    for (int c = 0; c < S::CHUNKS; ++c) {
+      float* buf = join + (S::JOIN_BUFS == 2 ? (c & 1) * S::JOIN : 0);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float(&o)[4] = w.o[c * 4 + t];
+        float* dst = buf + (warp * S::ROWS + g) * S::JOIN_ROW + t * 8 + quad * 2;
+        if constexpr (S::ROWS == 8) {
+          *reinterpret_cast<float2*>(dst) = make_float2((o[0] + o[2]) * mine_by[0], (o[1] + o[3]) * mine_by[0]);
+        } else {
+          *reinterpret_cast<float2*>(dst) = make_float2(o[0] * mine_by[0], o[1] * mine_by[0]);
+          *reinterpret_cast<float2*>(dst + 8 * S::JOIN_ROW) =
+              make_float2(o[2] * mine_by[Warp<S>::R - 1], o[3] * mine_by[Warp<S>::R - 1]);
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < S::RPT; ++i) {
+        const int row = warp + i * S::NW;
+        float v = 0.0f;
+#pragma unroll
+        for (int u = 0; u < S::NW; ++u) v += buf[(u * S::ROWS + row) * S::JOIN_ROW + lane];
+        sum[i][c] = v;
+      }
+      if (S::JOIN_BUFS == 1) __syncthreads();
+    }
+
+    const int n_tiles = at.live.tiles;
+    if (at.count == n_tiles) {              // the whole item
+#pragma unroll
+      for (int i = 0; i < S::RPT; ++i)
+        finish_row<S>(p, at.b, at.item, warp + i * S::NW, sum[i], row_m[i], row_l[i], lane);
+      continue;
+    }
+
+    // A share: to the workspace, slot 2c for an item that began in an earlier
+    // CTA, 2c + 1 for one that begins here.
+    const size_t slot = 2 * static_cast<size_t>(cta) + (at.t0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int i = 0; i < S::RPT; ++i) {
+      const int row = warp + i * S::NW;
+      float* dst = p.share_o + (slot * kMaxRows + row) * kMaxDim + lane;
+#pragma unroll
+      for (int c = 0; c < S::CHUNKS; ++c) dst[c * 32] = sum[i][c];
+      if (lane == 0) p.share_ml[slot * kMaxRows + row] = make_float2(row_m[i], row_l[i]);
+    }
+    // The CTAs of the item: those that own its first and its last tile.
+    const int c0 = static_cast<int>(((at.item_g0 + 1) * used - 1) / total);
+    const int c1 = static_cast<int>(((at.item_g0 + n_tiles) * used - 1) / total);
+    const int n = c1 - c0 + 1;
+    __syncthreads();
+    if (tid == 0) {
+      __threadfence();
+      const int seen = dg::sm100::atomic_add_acq_rel_gpu(p.tickets + c0, 1);
+      is_last = seen == n - 1;
+      if (seen == n - 1) dg::sm100::store_relaxed_gpu(p.tickets + c0, 0);   // ready for the next launch
+      __threadfence();
+    }
+    __syncthreads();
+    if (is_last == 0) continue;
+
+    // Join the shares, in CTA order.
+    float* by = join;                       // [ROWS][kMaxCtas] weights
+#pragma unroll
+    for (int i = 0; i < S::RPT; ++i) {
+      const int row = warp + i * S::NW;
+      float top = kNegInf;
+      for (int c = lane; c < n; c += 32) {
+        const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
+        top = fmaxf(top, __ldcg(p.share_ml + from * kMaxRows + row).x);
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      float l = 0.0f;
+      for (int c = lane; c < n; c += 32) {
+        const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
+        const float2 ml = __ldcg(p.share_ml + from * kMaxRows + row);
+        const float f = ml.x == kNegInf ? 0.0f : dg::warp::exp2_approx(ml.x - top);
+        by[row * kMaxCtas + c] = f;
+        l += f * ml.y;
+      }
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
+      __syncwarp();
+      float v[S::CHUNKS];
+#pragma unroll
+      for (int c = 0; c < S::CHUNKS; ++c) v[c] = 0.0f;
+#pragma unroll 4
+      for (int c = 0; c < n; ++c) {
+        const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
+        const float* src = p.share_o + (from * kMaxRows + row) * kMaxDim + lane;
+        const float f = by[row * kMaxCtas + c];
+#pragma unroll
+        for (int k = 0; k < S::CHUNKS; ++k) v[k] += f * __ldcg(src + k * 32);
+      }
+      finish_row<S>(p, at.b, at.item, row, v, top, l, lane);
+    }
+    __syncthreads();                        // the join buffers and is_last are free again
+  }
+  dg::warp::cp_async_wait<0>();
+}
+
+using Kernel = void (*)(const Params);
+
+struct Entry {
+  Kernel fn;
+  size_t smem;
+  int threads, rows;
+  std::atomic<unsigned long long> ready;    // per device: shared memory limit raised
+};
+
+template <typename S>
+Entry& entry() {
+  static Entry e{attention_kernel<S>, S::SMEM, S::NW * 32, S::ROWS, {0}};
+  return e;
+}
+
+template <typename MM, bool E4M3, int DP>
+Entry& pick_rows(bool few) {
+  return few ? entry<Shape<MM, E4M3, DP, 8>>() : entry<Shape<MM, E4M3, DP, 16>>();
+}
+
+Entry& pick(const dg_attention_args& a, bool few) {
+  const int d = a.head_dim;
+  if (a.cache_type == DG_TYPE_E4M3) return d <= 128 ? pick_rows<Fp16, true, 128>(few) : pick_rows<Fp16, true, 256>(few);
+  if (a.cache_type == DG_TYPE_FP16)
+    return d <= 64 ? pick_rows<Fp16, false, 64>(few)
+                   : d <= 128 ? pick_rows<Fp16, false, 128>(few) : pick_rows<Fp16, false, 256>(few);
+  return d <= 64 ? pick_rows<Bf16, false, 64>(few)
+                 : d <= 128 ? pick_rows<Bf16, false, 128>(few) : pick_rows<Bf16, false, 256>(few);
+}
+
+bool refused(const dg_attention_args& a) {
+  if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads != 0 || a.page_size < 1 ||
+      a.num_pages < 1 || a.table_width < 1 || a.table_stride < a.table_width || a.window < 0)
+    return true;
+  if (a.type != DG_TYPE_BF16 && a.type != DG_TYPE_FP16) return true;
+  const bool e4m3 = a.cache_type == DG_TYPE_E4M3;
+  if (!e4m3 && a.cache_type != a.type) return true;
+  if (a.head_dim < 8 || a.head_dim > kMaxDim || a.head_dim % (e4m3 ? 16 : 8) != 0) return true;
+  if (a.q == nullptr || a.k_cache == nullptr || a.v_cache == nullptr || a.block_table == nullptr ||
+      a.seq_lens == nullptr || a.out == nullptr || a.workspace == nullptr)
+    return true;
+  if (!e4m3 && (a.k_scale != nullptr || a.v_scale != nullptr)) return true;
+  if (!(a.softcap >= 0.0f) || !(a.scale == a.scale)) return true;
+  if ((reinterpret_cast<uintptr_t>(a.q) & 3u) != 0 || a.q_stride[0] % 2 != 0 || a.q_stride[1] % 2 != 0) return true;
+  if (((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u) != 0) return true;
+  for (int i = 0; i < 3; ++i)
+    if (a.k_cache_stride[i] % (e4m3 ? 16 : 8) != 0 || a.v_cache_stride[i] % (e4m3 ? 16 : 8) != 0) return true;
+  if ((a.q_out != nullptr) != (a.q_scales != nullptr)) return true;
+  if (a.q_out != nullptr && (a.head_dim % 128 != 0 || a.type != DG_TYPE_BF16)) return true;
+  if (a.workspace_bytes < kWorkspaceBytes || (reinterpret_cast<uintptr_t>(a.workspace) & 15u) != 0) return true;
+  // Items a request and tiles an item stay within ints.
+  if (static_cast<long long>(a.heads) > (1 << 20)) return true;
+  return false;
+}
+
+}  // namespace
+
+extern "C" {
+
+unsigned long long dg_attention_workspace_bytes(void) { return kWorkspaceBytes; }
+
+int dg_paged_attention(const dg_attention_args* args, void* stream, int pdl_attr) {
+  if (args == nullptr || refused(*args)) return cudaErrorInvalidValue;
+  Params p{};
+  p.a = *args;
+  p.group = p.a.heads / p.a.kv_heads;
+  Entry& e = pick(p.a, p.group <= 8);
+  p.groups = (p.group + e.rows - 1) / e.rows;
+  p.page_shift = -1;
+  if ((p.a.page_size & (p.a.page_size - 1)) == 0) {
+    p.page_shift = 0;
+    while ((1 << p.page_shift) < p.a.page_size) ++p.page_shift;
+  }
+  unsigned char* ws = static_cast<unsigned char*>(p.a.workspace);
+  p.tickets = reinterpret_cast<int*>(ws);
+  p.share_ml = reinterpret_cast<float2*>(ws + kTicketBytes);
+  p.share_o = reinterpret_cast<float*>(ws + kTicketBytes + kShares * kMaxRows * sizeof(float2));
+
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
+  const unsigned long long bit = 1ull << (dev & 63);
+  if ((e.ready.load(std::memory_order_acquire) & bit) == 0) {
+    err = cudaFuncSetAttribute(e.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(e.smem));
+    if (err != cudaSuccess) return err;
+    e.ready.fetch_or(bit, std::memory_order_release);
+  }
+  int ctas = dg_num_sms();
+  if (ctas < 1) ctas = 148;
+  if (ctas > kMaxCtas) ctas = kMaxCtas;
+
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr[1]{};
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(e.threads), 1, 1);
+  cfg.dynamicSmemBytes = e.smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;
+  if (pdl_attr) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, e.fn, p);
+}
+
+}  // extern "C"

@@ -13,6 +13,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "decode_attention_b200.h"
 #include "decode_gemm_b200.h"
 #include "dg_host.cuh"
 
@@ -643,6 +644,14 @@ const char* dg_status_string(int code) {
     case DG_ERR_BAD_LAUNCH_SHAPE: return "launch grid/block does not match the plan";
     case DG_ERR_REDUCE_WAIT: return "split reduction: a workspace bulk copy did not land in time";
     case DG_ERR_GATHER_WAIT: return "fused gather: a peer's output slices did not arrive in time";
+    case DG_ERR_LENGTH: return "block tables: a request length is negative or the sum is too large";
+    case DG_ERR_POOL: return "block tables: the free list has too few pages";
+    case DG_ERR_TABLE_WIDTH: return "block tables: a request needs more pages than its table row holds";
+    case DG_ERR_TOKENS: return "block tables: more new tokens than the output arrays hold";
+    case DG_ERR_POSITION: return "rotary: a position outside the cos/sin table";
+    case DG_ERR_SLOT: return "rotary: a slot past the end of the cache";
+    case DG_ERR_PAGE: return "paged attention: a page of a live token outside the cache";
+    case DG_ERR_SEQ_LEN: return "paged attention: a length outside the block table's row";
     default: return "unknown status";
   }
 }

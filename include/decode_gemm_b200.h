@@ -59,7 +59,7 @@
 extern "C" {
 #endif
 
-#define DG_ABI_VERSION 9
+#define DG_ABI_VERSION 10
 
 /* Weight layouts. */
 #define DG_LAYOUT_RAW 0             /* W[N,K], K contiguous (checkpoint layout) */
