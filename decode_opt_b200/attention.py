@@ -26,6 +26,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
@@ -48,43 +49,72 @@ def _need(ok: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _addr(t) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+def _addr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def _layout(struct_type) -> struct.Struct:
+    """A ctypes mirror as a struct.Struct of its members in order (arrays
+    spread out): packing one is ten times cheaper than filling the mirror, and
+    the calls of a decode step are short."""
+    code = {ctypes.c_int: "i", ctypes.c_uint: "I", ctypes.c_float: "f", ctypes.c_longlong: "q",
+            ctypes.c_ulonglong: "Q", ctypes.c_void_p: "P"}
+    form = "@"
+    for _, t in struct_type._fields_:
+        form += code[t] if t in code else f"{t._length_}{code[t._type_]}"
+    layout = struct.Struct(form)
+    assert layout.size <= ctypes.sizeof(struct_type) < layout.size + 8
+    # Trailing padding, so that the bytes are a whole C struct.
+    return struct.Struct(form + f"{ctypes.sizeof(struct_type) - layout.size}x")
+
+
+_PACK_TABLES = _layout(_lib.DgBlockTables).pack
+_PACK_ROTARY = _layout(_lib.DgRotaryArgs).pack
+_PACK_ATTENTION = _layout(_lib.DgAttentionArgs).pack
 
 
 @contextlib.contextmanager
 def _on(device, stream):
-    """With `device` current and, where one is given, `stream` too; yields the
-    stream's handle."""
+    """With `device` current and, where one is given, `stream` too."""
     with torch.cuda.device(device):
         if stream is None:
-            yield torch.cuda.current_stream(device).cuda_stream
+            yield
         else:
             s = torch.cuda.ExternalStream(stream, device=device) if isinstance(stream, int) else stream
             with torch.cuda.stream(s):
-                yield s.cuda_stream
+                yield
 
 
-def _launch(name: str, args, handle, pdl_attr) -> None:
-    rc = getattr(_lib.lib(), name)(ctypes.byref(args), handle, int(bool(pdl_attr)))
+def _elsewhere(device, stream) -> bool:
+    """Whether the call has to be made under :func:`_on` first."""
+    return stream is not None or torch.cuda.current_device() != device.index
+
+
+def _launch(name: str, args: bytes, device, pdl_attr) -> None:
+    rc = getattr(_lib.lib(), name)(args, torch._C._cuda_getCurrentRawStream(device.index), 1 if pdl_attr else 0)
     if rc != 0:
         raise RuntimeError(f"{name} failed: cudaError {rc}")
 
 
-def _check_same_device(device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, not {device}")
+def _check_ints(name: str, t, count: int, device, dtype=torch.int32) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != count or t.device != device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {count} values on {device}")
 
 
-def _check_ints(name: str, t, count: int, dtype=torch.int32) -> None:
-    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != count or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {count} values")
+def _check_status(status, device) -> None:
+    if status is not None and (status.dtype != torch.int32 or status.numel() < 1 or status.device != device):
+        raise ValueError(f"status must be an int32 tensor on {device}")
 
 
-def _check_status(status) -> None:
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
-        raise ValueError("status must be an int32 tensor")
+def _check_block_table(t, batch: int, device) -> Tuple[int, int]:
+    """(entries a row, row stride) of a block table."""
+    if t.dtype != torch.int32 or t.dim() != 2 or t.device != device:
+        raise ValueError(f"block_table must be int32 [{batch}, width] on {device}")
+    rows, width = t.shape
+    stride, unit = t.stride()
+    if rows != batch or width < 1 or (unit != 1 and width > 1) or (stride < width and batch > 1):
+        raise ValueError(f"block_table must be [{batch}, width >= 1] with unit column stride and rows that do not overlap")
+    return width, stride if batch > 1 else width
 
 
 # ---------------------------------------------------------------------------
@@ -118,43 +148,44 @@ def build_block_tables(context_lens, new_lens, free_pages, block_table, page_siz
     replayed for any smaller step.  `out` (a previous result of the same sizes)
     is written instead of new tensors."""
     _need(context_lens.is_cuda, "context_lens must be a CUDA tensor")
-    device, batch = context_lens.device, context_lens.shape[0]
+    device = context_lens.device
+    if _elsewhere(device, stream):
+        with _on(device, stream):
+            return build_block_tables(context_lens, new_lens, free_pages, block_table, page_size, num_tokens,
+                                      cursor=cursor, out=out, status=status, pdl_attr=pdl_attr)
+    batch, free_count = context_lens.shape[0], free_pages.shape[0]
     _need(1 <= batch <= 16384, "batch must be 1 .. 16384")
-    _check_ints("context_lens", context_lens, batch)
-    _check_ints("new_lens", new_lens, batch)
-    _check_ints("free_pages", free_pages, free_pages.shape[0])
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-          and block_table.shape[1] >= 1 and (block_table.stride(1) == 1 or block_table.shape[1] == 1),
-          "block_table must be int32 [batch, width], width >= 1, with unit column stride")
-    width = block_table.shape[1]
-    table_stride = block_table.stride(0) if batch > 1 else width
-    _need(table_stride >= width, "block_table's rows overlap")
+    _check_ints("context_lens", context_lens, batch, device)
+    _check_ints("new_lens", new_lens, batch, device)
+    _check_ints("free_pages", free_pages, free_count, device)
+    width, table_stride = _check_block_table(block_table, batch, device)
     _need(1 <= page_size <= _INT32_MAX and 0 <= num_tokens <= _INT32_MAX, "page_size >= 1 and num_tokens >= 0")
     if cursor is not None:
-        _check_ints("cursor", cursor, 1)
-    _check_status(status)
-    _check_same_device(device, new_lens=new_lens, free_pages=free_pages, block_table=block_table, cursor=cursor,
-                       status=status)
-    with _on(device, stream) as handle:
-        if out is None:
-            def ints(n, dtype=torch.int32):
-                return torch.empty(n, dtype=dtype, device=device)
-            out = StepTables(ints(batch), ints(batch + 1), ints(num_tokens, torch.int64), ints(num_tokens),
-                             ints(num_tokens), ints(1))
-        else:
-            _check_ints("out.seq_lens", out.seq_lens, batch)
-            _check_ints("out.query_start", out.query_start, batch + 1)
-            _check_ints("out.slots", out.slots, num_tokens, torch.int64)
-            _check_ints("out.positions", out.positions, num_tokens)
-            _check_ints("out.requests", out.requests, num_tokens)
-            _check_ints("out.cursor", out.cursor, 1)
-            _check_same_device(device, **vars(out))
-        args = _lib.DgBlockTables(batch, page_size, width, num_tokens, free_pages.shape[0], table_stride,
-                                  context_lens.data_ptr(), new_lens.data_ptr(), free_pages.data_ptr(), _addr(cursor),
-                                  block_table.data_ptr(), out.seq_lens.data_ptr(), out.query_start.data_ptr(),
-                                  out.slots.data_ptr(), out.positions.data_ptr(), out.requests.data_ptr(),
-                                  out.cursor.data_ptr(), _addr(status))
-        _launch("dg_build_block_tables", args, handle, pdl_attr)
+        _check_ints("cursor", cursor, 1, device)
+    _check_status(status, device)
+    if out is None:
+        # One allocation: 8-byte slots, then the 4-byte parts, each begun on 16 bytes.
+        tokens, rows, starts = (num_tokens + 3) & ~3, (batch + 3) & ~3, (batch + 4) & ~3
+        part = torch.empty(4 * tokens + rows + starts + 4, dtype=torch.int32, device=device)
+        slots, positions, requests, seq_lens, query_start, next_page = part.split_with_sizes(
+            (2 * tokens, tokens, tokens, rows, starts, 4))
+        slots = slots.view(torch.int64)
+        if tokens != num_tokens:
+            slots, positions, requests = slots[:num_tokens], positions[:num_tokens], requests[:num_tokens]
+        out = StepTables(seq_lens if rows == batch else seq_lens[:batch], query_start[:batch + 1], slots, positions,
+                         requests, next_page[:1])
+    else:
+        _check_ints("out.seq_lens", out.seq_lens, batch, device)
+        _check_ints("out.query_start", out.query_start, batch + 1, device)
+        _check_ints("out.slots", out.slots, num_tokens, device, torch.int64)
+        _check_ints("out.positions", out.positions, num_tokens, device)
+        _check_ints("out.requests", out.requests, num_tokens, device)
+        _check_ints("out.cursor", out.cursor, 1, device)
+    args = _PACK_TABLES(batch, page_size, width, num_tokens, free_count, table_stride, context_lens.data_ptr(),
+                        new_lens.data_ptr(), free_pages.data_ptr(), _addr(cursor), block_table.data_ptr(),
+                        out.seq_lens.data_ptr(), out.query_start.data_ptr(), out.slots.data_ptr(),
+                        out.positions.data_ptr(), out.requests.data_ptr(), out.cursor.data_ptr(), _addr(status))
+    _launch("dg_build_block_tables", args, device, pdl_attr)
     return out
 
 
@@ -190,32 +221,36 @@ def _axis_words(sections: Optional[Tuple[int, ...]], interleaved: bool, half: in
     words = [0] * (_lib.MAX_ROT // 32)
     for i, a in enumerate(axes):
         words[i // 16] |= a << (2 * (i % 16))
-    return len(sections), (ctypes.c_uint * len(words))(*words)
+    return len(sections), tuple(words)
 
 
 def _heads_of(name: str, t, tokens: int, dim: int, dtype, device):
-    if t.dim() != 3 or t.shape[0] != tokens or t.shape[2] != dim or t.dtype != dtype or t.device != device or \
-            t.stride(2) != 1:
-        raise ValueError(f"{name} must be {dtype} [{tokens}, heads, {dim}] on {device} with unit last stride")
+    """(heads, (token stride, head stride)) of a [tokens, heads, dim] tensor."""
+    if t.dim() != 3 or t.dtype != dtype or t.device != device:
+        raise ValueError(f"{name} must be {dtype} [{tokens}, heads, {dim}] on {device}")
+    n, heads, d = t.shape
+    s0, s1, unit = t.stride()
+    if n != tokens or d != dim or heads < 1 or unit != 1:
+        raise ValueError(f"{name} must be [{tokens}, heads >= 1, {dim}] with unit last stride")
+    return heads, (s0, s1)
 
 
-def _check_cache(k_cache, v_cache, heads: int, dim: int, dtype, device) -> int:
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if c.dim() != 4 or c.shape[2] != heads or c.shape[3] != dim or c.stride(3) != 1 or c.device != device:
-            raise ValueError(f"{name} must be [pages, page_size, {heads}, {dim}] on {device} with unit last stride")
-    if k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
-        raise ValueError("k_cache and v_cache must have one shape and type")
-    code = _CACHE_TYPE.get(k_cache.dtype)
-    if code is None or (code != _lib.TYPE_E4M3 and k_cache.dtype != dtype):
-        raise ValueError(f"the cache must be {dtype} or e4m3 (float8_e4m3fn or uint8), got {k_cache.dtype}")
-    if not (1 <= k_cache.shape[0] <= _INT32_MAX and k_cache.shape[1] >= 1):
-        raise ValueError("the cache needs at least one page of one token")
-    return code
+def _cache_of(k_cache, v_cache, heads: int, dim: int, dtype, device):
+    """(type, pages, page size, strides of k_cache, strides of v_cache)."""
+    kind = k_cache.dtype
+    code = _CACHE_TYPE.get(kind)
+    if code is None or (code != _lib.TYPE_E4M3 and kind != dtype) or v_cache.dtype != kind:
+        raise ValueError(f"both caches must be {dtype} or e4m3 (float8_e4m3fn or uint8), got {kind}, {v_cache.dtype}")
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
+    if len(shape) != 4 or v_cache.shape != shape or k_cache.device != device or v_cache.device != device:
+        raise ValueError(f"both caches must be [pages, page_size, {heads}, {dim}] on {device}")
+    pages, page_size, h, d = shape
+    if h != heads or d != dim or ks[3] != 1 or vs[3] != 1 or not 1 <= pages <= _INT32_MAX or page_size < 1:
+        raise ValueError(f"the caches must be [pages >= 1, page_size >= 1, {heads}, {dim}] with unit last stride")
+    return code, pages, page_size, ks[:3], vs[:3]
 
 
 def _check_scale(name: str, t, heads: int, code: int, device) -> None:
-    if t is None:
-        return
     if code != _lib.TYPE_E4M3:
         raise ValueError(f"{name} goes with an e4m3 cache")
     if t.dtype != torch.float32 or t.dim() != 1 or t.shape[0] != heads or not t.is_contiguous() or t.device != device:
@@ -226,74 +261,72 @@ _NO2, _NO3 = (0, 0), (0, 0, 0)
 
 
 def _rotary(q, k, v, positions, table, sections, interleaved, pairing, inverse, q_out, k_out, caches, slots, k_scale,
-            v_scale, status, stream, pdl_attr):
-    """dg_rotary; returns (q_out, k_out), made here where they are True."""
+            v_scale, status, pdl_attr):
+    """dg_rotary on the current device and stream; returns (q_out, k_out), made
+    here where they are True."""
     x = q if q is not None else k
-    _need(x is not None and x.is_cuda, "q or k must be a CUDA tensor")
-    _need(x.dim() == 3 and x.shape[0] >= 1 and x.dtype in _TYPE, "q and k must be bf16, fp16 or fp32 [tokens, heads, dim]")
-    device, dtype = x.device, x.dtype
+    dtype, device = x.dtype, x.device
+    kind = _TYPE.get(dtype)
+    _need(kind is not None and x.dim() == 3 and x.shape[0] >= 1,
+          "q and k must be bf16, fp16 or fp32 [tokens >= 1, heads, dim]")
     tokens, _, dim = x.shape
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if t is not None:
-            _heads_of(name, t, tokens, dim, dtype, device)
-    _need(table.dtype == torch.float32 and table.dim() == 2 and table.is_contiguous() and table.device == device,
-          f"table must be a contiguous fp32 [max_position, rot] tensor on {device}")
+    heads = kv_heads = code = pages = page_size = 0
+    qs = ks = vs = qos = kos = _NO2
+    kcs = vcs = _NO3
+    if q is not None:
+        heads, qs = _heads_of("q", q, tokens, dim, dtype, device)
+    if k is not None:
+        kv_heads, ks = _heads_of("k", k, tokens, dim, dtype, device)
+    if table.dtype != torch.float32 or table.dim() != 2 or table.device != device or not table.is_contiguous():
+        raise ValueError(f"table must be a contiguous fp32 [max_position, rot] tensor on {device}")
     max_position, rot = table.shape
-    _need(max_position >= 1 and 2 <= rot <= min(dim, _lib.MAX_ROT) and rot % 2 == 0,
-          f"the table's width must be even and at most {min(dim, _lib.MAX_ROT)}")
+    if max_position < 1 or rot < 2 or rot % 2 != 0 or rot > dim or rot > _lib.MAX_ROT:
+        raise ValueError(f"the table's width must be even and at most {min(dim, _lib.MAX_ROT)}")
     _need(pairing in _PAIRING, "pairing must be 'half' or 'adjacent'")
     axes, words = _axis_words(None if sections is None else tuple(sections), bool(interleaved), rot // 2)
-    _need(positions.dtype in (torch.int32, torch.int64) and positions.device == device
-          and positions.dim() in (1, 2) and positions.shape[-1] == tokens
-          and (positions.stride(-1) == 1 or tokens == 1),
-          f"positions must be int32 or int64 [{tokens}] or [axes, {tokens}] on {device}")
+    wide = positions.dtype == torch.int64
+    shape, strides = positions.shape, positions.stride()
+    if not (wide or positions.dtype == torch.int32) or positions.device != device or len(shape) not in (1, 2) or \
+            shape[-1] != tokens or (strides[-1] != 1 and tokens > 1):
+        raise ValueError(f"positions must be int32 or int64 [{tokens}] or [axes, {tokens}] on {device}")
     position_stride = 0
-    if positions.dim() == 2:
-        _need(positions.shape[0] == axes, f"positions has {positions.shape[0]} axes, the sections {axes}")
-        position_stride = positions.stride(0) if axes > 1 else 0
+    if len(shape) == 2:
+        _need(shape[0] == axes, f"positions has {shape[0]} axes, the sections {axes}")
+        position_stride = strides[0] if axes > 1 else 0
         _need(position_stride >= 0, "positions must not run backwards")
-    _check_status(status)
-    _check_same_device(device, status=status)
-    heads = 0 if q is None else q.shape[1]
-    kv_heads = 0 if k is None else k.shape[1]
-    _need((q is None or heads >= 1) and (k is None or kv_heads >= 1), "q and k need at least one head")
-    code = pages = page_size = 0
+    if status is not None:
+        _check_status(status, device)
     k_cache = v_cache = None
     if caches is not None:
         k_cache, v_cache = caches
-        _need(k.shape == v.shape, "k and v must have one shape")
+        v_heads, vs = _heads_of("v", v, tokens, dim, dtype, device)
+        _need(v_heads == kv_heads, "k and v must have one shape")
         _need(dtype != torch.float32, "the cache write takes bf16 or fp16")
-        code = _check_cache(k_cache, v_cache, kv_heads, dim, dtype, device)
-        pages, page_size = k_cache.shape[:2]
-        _check_ints("slots", slots, tokens, torch.int64)
-        _check_same_device(device, slots=slots)
-        _check_scale("k_scale", k_scale, kv_heads, code, device)
-        _check_scale("v_scale", v_scale, kv_heads, code, device)
-    for name, t, like in (("out_q", q_out, q), ("out_k", k_out, k)):
-        if isinstance(t, torch.Tensor):
-            _need(like is not None, f"{name} without its input")
-            _heads_of(name, t, tokens, dim, dtype, device)
-            _need(t.shape == like.shape, f"{name} must have its input's shape")
-    with _on(device, stream) as handle:
-        if q_out is True:
-            q_out = torch.empty(q.shape, dtype=dtype, device=device)
-        if k_out is True:
-            k_out = torch.empty(k.shape, dtype=dtype, device=device)
-
-        def two(t):
-            return _NO2 if t is None else t.stride()[:2]
-
-        def three(t):
-            return _NO3 if t is None else t.stride()[:3]
-
-        args = _lib.DgRotaryArgs(
-            tokens, heads, kv_heads, dim, rot, _TYPE[dtype], code if caches is not None else _TYPE[dtype],
-            _PAIRING[pairing], int(bool(inverse)), int(positions.dtype == torch.int64), max_position, page_size, pages,
-            _addr(q), _addr(k), _addr(v), _addr(q_out), _addr(k_out), _addr(k_cache), _addr(v_cache),
-            two(q), two(k), two(v), two(q_out), two(k_out), three(k_cache), three(v_cache),
-            positions.data_ptr(), position_stride, _addr(slots), table.data_ptr(), _addr(k_scale), _addr(v_scale),
-            _addr(status), words)
-        _launch("dg_rotary", args, handle, pdl_attr)
+        code, pages, page_size, kcs, vcs = _cache_of(k_cache, v_cache, kv_heads, dim, dtype, device)
+        _check_ints("slots", slots, tokens, device, torch.int64)
+        if k_scale is not None:
+            _check_scale("k_scale", k_scale, kv_heads, code, device)
+        if v_scale is not None:
+            _check_scale("v_scale", v_scale, kv_heads, code, device)
+    if q_out is True:
+        q_out, qos = torch.empty((tokens, heads, dim), dtype=dtype, device=device), (heads * dim, dim)
+    elif q_out is not None:
+        _need(q is not None, "out_q without q")
+        n, qos = _heads_of("out_q", q_out, tokens, dim, dtype, device)
+        _need(n == heads, "out_q must have q's shape")
+    if k_out is True:
+        k_out, kos = torch.empty((tokens, kv_heads, dim), dtype=dtype, device=device), (kv_heads * dim, dim)
+    elif k_out is not None:
+        _need(k is not None, "out_k without k")
+        n, kos = _heads_of("out_k", k_out, tokens, dim, dtype, device)
+        _need(n == kv_heads, "out_k must have k's shape")
+    args = _PACK_ROTARY(
+        tokens, heads, kv_heads, dim, rot, kind, code if caches is not None else kind, _PAIRING[pairing],
+        1 if inverse else 0, 1 if wide else 0, max_position, page_size, pages, _addr(q), _addr(k), _addr(v),
+        _addr(q_out), _addr(k_out), _addr(k_cache), _addr(v_cache), *qs, *ks, *vs, *qos, *kos, *kcs, *vcs,
+        positions.data_ptr(), position_stride, _addr(slots), table.data_ptr(), _addr(k_scale), _addr(v_scale),
+        _addr(status), *words)
+    _launch("dg_rotary", args, device, pdl_attr)
     return q_out, k_out
 
 
@@ -305,20 +338,20 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, positions, table, kw):
         ctx.save_for_backward(positions, table)
         ctx.kw = kw
-        return _rotary(q, k, None, positions, table, *kw[:3], kw[3], q is not None or None, k is not None or None, None,
-                       None, None, None, *kw[4:])
+        sections, interleaved, pairing, inverse, status, pdl_attr = kw
+        return _rotary(q, k, None, positions, table, sections, interleaved, pairing, inverse, q is not None or None,
+                       k is not None or None, None, None, None, None, status, pdl_attr)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, table = ctx.saved_tensors
-        kw = ctx.kw
+        sections, interleaved, pairing, inverse = ctx.kw[:4]
         dq, dk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
         gq = gk = None
         if dq is not None or dk is not None:
-            # On the stream and with the status of the moment, not of the forward pass.
-            gq, gk = _rotary(dq, dk, None, positions, table, *kw[:3], not kw[3], dq is not None or None,
-                             dk is not None or None, None, None, None, None, None, None, False)
+            gq, gk = _rotary(dq, dk, None, positions, table, sections, interleaved, pairing, not inverse,
+                             dq is not None or None, dk is not None or None, None, None, None, None, None, False)
         return gq, gk, None, None, None
 
 
@@ -335,14 +368,19 @@ def rotary(q, k, positions, table, *, sections: Optional[Sequence[int]] = None, 
     turn (``interleaved``) while an axis has pairs left.  ``inverse`` turns
     back, which is also the gradient; the call is differentiable in q and k.
     `out_q`, `out_k` may be q and k themselves."""
-    kw = (sections, interleaved, pairing, inverse, status, stream, pdl_attr)
+    x = q if q is not None else k
+    _need(x is not None and x.is_cuda, "q or k must be a CUDA tensor")
+    if _elsewhere(x.device, stream):
+        with _on(x.device, stream):
+            return rotary(q, k, positions, table, sections=sections, interleaved=interleaved, pairing=pairing,
+                          inverse=inverse, out_q=out_q, out_k=out_k, status=status, pdl_attr=pdl_attr)
     if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
         _need(out_q is None and out_k is None, "out_q and out_k do not go with a gradient")
-        return _Rotary.apply(q, k, positions, table, kw)
+        return _Rotary.apply(q, k, positions, table, (sections, interleaved, pairing, inverse, status, pdl_attr))
     return _rotary(q, k, None, positions, table, sections, interleaved, pairing, inverse,
                    out_q if out_q is not None else (True if q is not None else None),
                    out_k if out_k is not None else (True if k is not None else None),
-                   None, None, None, None, status, stream, pdl_attr)
+                   None, None, None, None, status, pdl_attr)
 
 
 def rotary_append(q, k, v, positions, slots, k_cache, v_cache, table, *, sections: Optional[Sequence[int]] = None,
@@ -356,10 +394,15 @@ def rotary_append(q, k, v, positions, slots, k_cache, v_cache, table, *, section
     scale[head], +-448))`` is stored, `k_scale` and `v_scale` fp32 [Hk] or None
     for 1.  ``slots[t] = page * page_size + offset`` (int64; below 0: the token
     is not cached).  Slots of one call must differ."""
-    _need(q is not None and k is not None and v is not None, "rotary_append takes q, k and v")
+    _need(q is not None and k is not None and v is not None and q.is_cuda, "rotary_append takes CUDA tensors q, k and v")
+    if _elsewhere(q.device, stream):
+        with _on(q.device, stream):
+            return rotary_append(q, k, v, positions, slots, k_cache, v_cache, table, sections=sections,
+                                 interleaved=interleaved, pairing=pairing, k_scale=k_scale, v_scale=v_scale,
+                                 out_q=out_q, status=status, pdl_attr=pdl_attr)
     return _rotary(q, k, v, positions, table, sections, interleaved, pairing, False,
                    out_q if out_q is not None else True, None, (k_cache, v_cache), slots, k_scale, v_scale, status,
-                   stream, pdl_attr)[0]
+                   pdl_attr)[0]
 
 
 # ---------------------------------------------------------------------------
@@ -370,21 +413,25 @@ _ATTENTION_WORKSPACES: dict = {}
 _TICKET_BYTES = 1024
 
 
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes() -> int:
+    return int(_lib.lib().dg_attention_workspace_bytes())
+
+
 def attention_workspace(device="cuda") -> torch.Tensor:
     """A workspace for :func:`paged_attention` (about 5 MB, any arguments).
     Calls that can overlap on the GPU need one each."""
-    nbytes = int(_lib.lib().dg_attention_workspace_bytes())
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    ws = torch.empty(_workspace_bytes(), dtype=torch.uint8, device=device)
     ws[:_TICKET_BYTES].zero_()               # the tickets; the rest is written before it is read
     return ws
 
 
-def _stream_workspace(device, handle) -> torch.Tensor:
+def _stream_workspace(device) -> torch.Tensor:
     # Kept per stream: calls on one stream run one after another.  A captured
     # graph may be replayed on any stream, so it gets its own, from its pool.
     if torch.cuda.is_current_stream_capturing():
         return attention_workspace(device)
-    key = (device.index, handle)
+    key = (device.index, torch._C._cuda_getCurrentRawStream(device.index))
     ws = _ATTENTION_WORKSPACES.get(key)
     if ws is None:
         ws = _ATTENTION_WORKSPACES[key] = attention_workspace(device)
@@ -412,61 +459,64 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: Option
     ``quantize_activation`` (bf16 and D a multiple of 128).  `workspace`: from
     :func:`attention_workspace`; by default one is kept per stream, and a call
     under capture gets its own, zeroed in the graph."""
-    _need(q.is_cuda and q.dim() == 3 and q.dtype in (torch.bfloat16, torch.float16) and q.stride(2) == 1
-          and q.shape[0] >= 1, "q must be bf16 or fp16 [batch >= 1, heads, dim] on a GPU with unit last stride")
+    _need(q.is_cuda and q.dim() == 3, "q must be a CUDA tensor [batch, heads, dim]")
     device, dtype = q.device, q.dtype
+    if _elsewhere(device, stream):
+        with _on(device, stream):
+            return paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale=scale, window=window,
+                                   softcap=softcap, k_scale=k_scale, v_scale=v_scale, out=out, return_lse=return_lse,
+                                   q_out=q_out, q_scales=q_scales, workspace=workspace, status=status,
+                                   pdl_attr=pdl_attr)
+    _need(dtype == torch.bfloat16 or dtype == torch.float16, "q must be bf16 or fp16")
     batch, heads, dim = q.shape
-    _need(k_cache.dim() == 4, "k_cache must be [pages, page_size, kv_heads, dim]")
+    q0, q1, unit = q.stride()
+    q_at, k_at, v_at = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    _need(batch >= 1 and unit == 1 and (q_at | 2 * q0 | 2 * q1) % 4 == 0,
+          "q must be [batch >= 1, heads, dim], 4-byte aligned, with unit last and otherwise even strides")
+    _need(k_cache.dim() == 4, "the caches must be [pages, page_size, kv_heads, dim]")
     kv_heads = k_cache.shape[2]
     _need(kv_heads >= 1 and heads >= 1 and heads % kv_heads == 0, "heads must be a multiple of the cache's heads")
-    code = _check_cache(k_cache, v_cache, kv_heads, dim, dtype, device)
-    unit = 16 if code == _lib.TYPE_E4M3 else 8
+    code, pages, page_size, ks, vs = _cache_of(k_cache, v_cache, kv_heads, dim, dtype, device)
+    unit = 16 if code == _lib.TYPE_E4M3 else 8       # 16 bytes
     _need(8 <= dim <= 256 and dim % unit == 0, f"dim must be a multiple of {unit}, at most 256")
-    qs, ks, vs = q.stride(), k_cache.stride(), v_cache.stride()
-    _need(qs[0] % 2 == 0 and qs[1] % 2 == 0 and q.data_ptr() % 4 == 0, "q must be 4-byte aligned with even strides")
-    _need(ks[0] % unit == 0 and ks[1] % unit == 0 and ks[2] % unit == 0 and vs[0] % unit == 0 and vs[1] % unit == 0
-          and vs[2] % unit == 0 and (k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0,
+    _need((ks[0] | ks[1] | ks[2] | vs[0] | vs[1] | vs[2]) % unit == 0 and (k_at | v_at) % 16 == 0,
           "the caches must be 16-byte aligned, strides multiples of 16 bytes")
-    _need(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == batch
-          and block_table.shape[1] >= 1 and (block_table.stride(1) == 1 or block_table.shape[1] == 1)
-          and block_table.device == device,
-          f"block_table must be int32 [{batch}, width >= 1] on {device} with unit column stride")
-    width = block_table.shape[1]
-    table_stride = block_table.stride(0) if batch > 1 else width
-    _need(table_stride >= width, "block_table's rows overlap")
-    _check_ints("seq_lens", seq_lens, batch)
-    _check_scale("k_scale", k_scale, kv_heads, code, device)
-    _check_scale("v_scale", v_scale, kv_heads, code, device)
+    width, table_stride = _check_block_table(block_table, batch, device)
+    _check_ints("seq_lens", seq_lens, batch, device)
+    if k_scale is not None:
+        _check_scale("k_scale", k_scale, kv_heads, code, device)
+    if v_scale is not None:
+        _check_scale("v_scale", v_scale, kv_heads, code, device)
     _need(window is None or 1 <= window <= _INT32_MAX, "window must be at least 1")
     _need(softcap is None or 0.0 < softcap < float("inf"), "softcap must be positive")
-    _check_status(status)
-    _check_same_device(device, seq_lens=seq_lens, workspace=workspace, status=status)
+    if status is not None:
+        _check_status(status, device)
     if out is not None:
-        _heads_of("out", out, batch, dim, dtype, device)
-        _need(out.shape == q.shape, "out must have q's shape")
+        n, (o0, o1) = _heads_of("out", out, batch, dim, dtype, device)
+        _need(n == heads, "out must have q's shape")
     if q_out is not None or q_scales is not None:
         _need(q_out is not None and q_scales is not None, "q_out and q_scales go together")
         _need(dtype == torch.bfloat16 and dim % 128 == 0, "the quantised result takes bf16 and dim a multiple of 128")
         n = heads * dim
-        _need(q_out.dtype in (torch.uint8, torch.float8_e4m3fn) and tuple(q_out.shape) == (batch, n)
+        _need(q_out.dtype in (torch.uint8, torch.float8_e4m3fn) and q_out.shape == (batch, n)
               and q_out.is_contiguous() and q_out.device == device, f"q_out must be uint8 [{batch}, {n}], contiguous")
-        _need(q_scales.dtype == torch.float32 and tuple(q_scales.shape) == (batch, n // 128)
+        _need(q_scales.dtype == torch.float32 and q_scales.shape == (batch, n // 128)
               and q_scales.is_contiguous() and q_scales.device == device,
               f"q_scales must be fp32 [{batch}, {n // 128}], contiguous")
-    if workspace is not None:
-        _need(workspace.is_contiguous() and workspace.data_ptr() % 16 == 0
-              and workspace.numel() * workspace.element_size() >= _lib.lib().dg_attention_workspace_bytes(),
-              "workspace must come from attention_workspace()")
-    with _on(device, stream) as handle:
-        if out is None:
-            out = torch.empty((batch, heads, dim), dtype=dtype, device=device)
-        lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
-        ws = workspace if workspace is not None else _stream_workspace(device, handle)
-        args = _lib.DgAttentionArgs(
-            batch, heads, kv_heads, dim, k_cache.shape[1], k_cache.shape[0], width, _TYPE[dtype], code, window or 0,
-            dim ** -0.5 if scale is None else scale, softcap or 0.0, q.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), qs[:2], ks[:3], vs[:3], block_table.data_ptr(), table_stride, seq_lens.data_ptr(),
-            _addr(k_scale), _addr(v_scale), out.data_ptr(), out.stride()[:2], _addr(lse), _addr(q_out),
-            _addr(q_scales), ws.data_ptr(), ws.numel() * ws.element_size(), _addr(status))
-        _launch("dg_paged_attention", args, handle, pdl_attr)
+    nbytes = _workspace_bytes()
+    if workspace is None:
+        workspace = _stream_workspace(device)
+    else:
+        _need(workspace.device == device and workspace.is_contiguous() and workspace.data_ptr() % 16 == 0
+              and workspace.numel() * workspace.element_size() >= nbytes,
+              f"workspace must come from attention_workspace({str(device)!r})")
+    if out is None:
+        out, o0, o1 = torch.empty((batch, heads, dim), dtype=dtype, device=device), heads * dim, dim
+    lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
+    args = _PACK_ATTENTION(
+        batch, heads, kv_heads, dim, page_size, pages, width, _TYPE[dtype], code, window or 0,
+        dim ** -0.5 if scale is None else scale, softcap or 0.0, q_at, k_at, v_at, q0, q1, *ks, *vs,
+        block_table.data_ptr(), table_stride, seq_lens.data_ptr(), _addr(k_scale), _addr(v_scale), out.data_ptr(), o0,
+        o1, _addr(lse), _addr(q_out), _addr(q_scales), workspace.data_ptr(), nbytes, _addr(status))
+    _launch("dg_paged_attention", args, device, pdl_attr)
     return (out, lse) if return_lse else out
