@@ -10,17 +10,19 @@
 //
 // Split.  The work is cut into tiles of TOK tokens of one (request, kv head,
 // group of ROWS query heads) "item"; all tiles of all items stand in one
-// line, and CTA c of G takes tiles [W c / G, W (c+1) / G) of it -- equal shares
-// whatever the lengths are, one CTA an SM.  The line is laid out on the
-// device from seq_lens (one scan of the batch per CTA), so that the host
-// needs no lengths.  A CTA therefore works on a run of items: the first and
-// the last may be shared with its neighbours, those between are its own.
-// Within an item's share the CTA's warps take tiles in turn, each with its
-// own ring of TOK-token stages filled by its own cp.async copies: no barrier
-// in the loop, and the ring runs on across items, so that the end of one
-// does not drain it.  16-byte copies with the row's address from the page
-// table (one table entry per token and lane, fetched a tile ahead) take any
-// page size and strides; tokens that are not live are zero-filled and masked.
+// line, each item preceded by the units that its beginning and end cost, and
+// CTA c of G takes units [U c / G, U (c+1) / G) of it -- equal shares whatever the
+// lengths are, one CTA an SM.  The line is laid out on the device from
+// seq_lens (one scan of the batch per CTA), so that the host needs no
+// lengths.  A CTA therefore works on a run of items: the first and the last
+// may be shared with its neighbours, those between are its own.  Within an
+// item's share the CTA's warps take tiles in turn; items of a few tiles are
+// done by one warp each, without the join.  Every warp has its own ring of
+// TOK-token stages filled by its own cp.async copies: no barrier in the loop,
+// and the ring runs on across items, so that the end of one does not drain
+// it.  16-byte copies with the row's address from the page table (one table
+// entry per token and lane, fetched a tile ahead) take any page size and
+// strides; tokens that are not live are zero-filled and masked.
 //
 // Products: mma.sync m16n8k16, the query heads as its 16 rows.  At 16 rows
 // the tensor pipe is far from its limit at HBM speed (43 bytes a ns and SM
@@ -107,6 +109,9 @@ struct Shape {
   static constexpr int JOIN_ROW = 40;                            // 32 columns, padded against bank conflicts
   static constexpr int JOIN_BUFS = ROWS_ == 8 ? 2 : 1;
   static constexpr int JOIN = NW * ROWS_ * JOIN_ROW;             // floats a buffer
+  static constexpr int SOLO = NW;                                // tiles of an item that one warp does alone
+  static constexpr int EXTRA_SOLO = 1, EXTRA = 8;                // an item's cost in tiles, beyond its tiles
+  static constexpr int MIN_RUN = 4;                              // units a CTA takes at least
   static constexpr int NT = TOK / 8;                             // score tiles of 8 tokens
   static constexpr int KS = DP_ / 16;                            // inner steps of Q K^T
   static constexpr int OT = DP_ / 8;                             // output tiles of 8 columns
@@ -137,14 +142,23 @@ __device__ __forceinline__ void report(int* status, int code) {
   if (status != nullptr) atomicCAS(status, 0, code);
 }
 
-// A request's live tokens as tiles.
+// a / b for a line that may be longer than 32 bits; it rarely is, and the
+// 32-bit division is a quarter of the instructions.
+__device__ __forceinline__ unsigned long long divided(unsigned long long a, unsigned long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+// A request's live tokens as tiles, and what one of its items costs beyond
+// them.
 struct Live {
   int lo, len;    // live tokens [lo, len)
   int first;      // first tile
   int tiles;      // tiles, 0 if nothing is live
+  int extra;      // units of the line before the item's first tile
 };
 
-template <int TOK>
+template <typename S>
 __device__ __forceinline__ Live live_of(const dg_attention_args& a, int b, bool tell) {
   Live v;
   int len = a.seq_lens[b];
@@ -155,58 +169,74 @@ __device__ __forceinline__ Live live_of(const dg_attention_args& a, int b, bool 
   }
   v.len = len;
   v.lo = a.window > 0 && len > a.window ? len - a.window : 0;
-  v.first = v.lo / TOK;
-  v.tiles = len > 0 ? (len - 1) / TOK + 1 - v.first : 0;
+  v.first = v.lo / S::TOK;
+  v.tiles = len > 0 ? (len - 1) / S::TOK + 1 - v.first : 0;
+  v.extra = v.tiles <= S::SOLO ? S::EXTRA_SOLO : S::EXTRA;
   return v;
 }
 
-// A place in a CTA's run of tiles: one item's share.
-template <int TOK>
+// A place in a CTA's run [x, x1) of the line: one item's share.
+template <typename S>
 struct Cursor {
-  long long g, g1;       // the share's first tile in the line, end of the CTA's run
-  long long item_g0;     // the item's first tile in the line
+  long long x1;          // end of the CTA's run
+  long long item_x0;     // the item's first unit
   int b, item;           // request, item of the request
   int t0, count;         // the share: tiles [t0, t0 + count) of the item
+  int turn;              // solo shares before this one
+  bool solo;             // one warp's work (turn % NW) instead of the CTA's
+  long long run;         // the run's units
   Live live;
 
-  __device__ __forceinline__ void settle() {
-    count = static_cast<int>(min(static_cast<long long>(live.tiles - t0), g1 - g));
+  // The share [t0, ...) of the item; false if the run ends before it.
+  __device__ __forceinline__ bool settle() {
+    const long long end = x1 - item_x0 - live.extra;
+    count = static_cast<int>(min(static_cast<long long>(live.tiles), end)) - t0;
+    // One warp takes as many steps as the item has tiles, but several items go
+    // side by side: worth it where the run holds more than the one.
+    solo = live.tiles <= S::SOLO && count == live.tiles && run >= 2 * (live.tiles + live.extra);
+    return count > 0;
   }
-  __device__ __forceinline__ void start(const dg_attention_args& a, int request, long long base, long long from,
+  __device__ __forceinline__ bool start(const dg_attention_args& a, int request, long long base, long long from,
                                         long long to) {
     b = request;
-    g = from;
-    g1 = to;
-    live = live_of<TOK>(a, b, false);
-    const long long off = from - base;
-    item = static_cast<int>(off / live.tiles);
-    t0 = static_cast<int>(off - static_cast<long long>(item) * live.tiles);
-    item_g0 = from - t0;
-    settle();
+    x1 = to;
+    run = to - from;
+    turn = 0;
+    live = live_of<S>(a, b, false);
+    const int units = live.tiles + live.extra;
+    const unsigned long long off = static_cast<unsigned long long>(from - base);
+    item = static_cast<int>(divided(off, static_cast<unsigned long long>(units)));
+    item_x0 = base + static_cast<long long>(item) * units;
+    t0 = max(0, static_cast<int>(from - item_x0) - live.extra);
+    return settle();
   }
   // To the next share; false at the end of the run.
   __device__ __forceinline__ bool advance(const dg_attention_args& a, int items) {
-    g += count;
-    if (g >= g1) return false;
+    item_x0 += live.tiles + live.extra;
+    if (item_x0 >= x1) return false;
+    if (solo) ++turn;
     if (++item == items) {
       item = 0;
       do {
-        ++b;             // g < g1 <= W: a later request has tiles
-        live = live_of<TOK>(a, b, false);
+        ++b;             // item_x0 < x1: a later request has tiles
+        live = live_of<S>(a, b, false);
       } while (live.tiles == 0);
     }
-    item_g0 = g;
     t0 = 0;
-    settle();
-    return true;
+    return settle();
   }
+  // This warp's tiles of the share: first, first + step, ...
+  __device__ __forceinline__ int first_tile(int warp) const {
+    return !solo ? warp : (turn % S::NW == warp ? 0 : count);
+  }
+  __device__ __forceinline__ int step() const { return solo ? 1 : S::NW; }
 };
 
 // One warp's copies: tile after tile of the CTA's run, ahead of the products.
 template <typename S>
 struct Loader {
-  Cursor<S::TOK> at;
-  int tile;              // of the share: warp, warp + NW, ...
+  Cursor<S> at;
+  int tile;              // of the share
   bool more;             // a tile is pending
   // The pending tile: this lane's token.
   int page, offset, head;
@@ -239,10 +269,10 @@ struct Loader {
         more = false;
         return;
       }
-      tile = warp;
+      tile = at.first_tile(warp);
     }
     look_up(p, lane);
-    tile += S::NW;
+    tile += at.step();
   }
   // Copies the pending tile into a stage.
   __device__ __forceinline__ void issue(const Params& p, uint32_t stage, uint32_t* mask, int lane) const {
@@ -584,6 +614,61 @@ __device__ __forceinline__ void finish_row(const Params& p, int b, int item, int
   }
 }
 
+// An item that this warp did alone, from its registers: 16 output tiles (128
+// columns) at a time, two values of each a lane.
+template <typename S>
+__device__ __forceinline__ void finish_solo(const Params& p, int b, int item, const Warp<S>& w, int lane) {
+  const dg_attention_args& a = p.a;
+  const int head = p.groups == 1 ? item : item / p.groups;
+  const int g = lane >> 2, quad = lane & 3;
+  const long long width = static_cast<long long>(a.heads) * a.head_dim;
+#pragma unroll
+  for (int r = 0; r < Warp<S>::R; ++r) {
+    float l = w.l[r];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const int in_group = (item - head * p.groups) * S::ROWS + g + 8 * r;
+    const bool real = in_group < p.group;
+    const int h = head * p.group + in_group;
+    float norm = 1.0f / l;
+    if (S::kE4m3 && a.v_scale != nullptr) norm *= a.v_scale[head];
+    const long long at = b * a.out_stride[0] + h * a.out_stride[1];
+    if (real && a.lse != nullptr && quad == 0)
+      a.lse[static_cast<long long>(b) * a.heads + h] = (w.m[r] - S::kBias) * kLn2 + logf(l);
+    constexpr int BLOCK = S::OT < 16 ? S::OT : 16;
+#pragma unroll
+    for (int t0 = 0; t0 < S::OT; t0 += BLOCK) {
+      float top = 0.0f;
+      float x[BLOCK][2];
+#pragma unroll
+      for (int t = 0; t < BLOCK; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float(&o)[4] = w.o[t0 + t];
+          const float v = (Warp<S>::R == 1 ? o[i] + o[2 + i] : o[2 * r + i]) * norm;
+          const int d = S::column(t0 + t, quad * 2 + i);
+          if (real && d < a.head_dim) store_out(a, at + d, v);
+          x[t][i] = __bfloat162float(__float2bfloat16_rn(v));
+          top = max_ref(top, fabsf(x[t][i]));
+        }
+      if (S::DP >= 128 && a.q_out != nullptr && t0 * 8 < a.head_dim) {
+        top = max_ref(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max_ref(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        if (!real) continue;
+        const float scale = max_ref(top, kQuantEps) / kFp8Max;
+        const long long q_at = b * width + static_cast<long long>(h) * a.head_dim;
+#pragma unroll
+        for (int t = 0; t < BLOCK; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            static_cast<uint8_t*>(a.q_out)[q_at + S::column(t0 + t, quad * 2 + i)] =
+                __nv_fp8_e4m3(min_ref(max_ref(x[t][i] / scale, -kFp8Max), kFp8Max)).__x;
+        if (quad == 0) a.q_scales[(q_at + t0 * 8) / 128] = scale;
+      }
+    }
+  }
+}
+
 template <typename S>
 __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -606,7 +691,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 
   // Requests without live tokens, dealt over the CTAs.
   for (int b = cta; b < a.batch; b += ctas) {
-    if (live_of<S::TOK>(a, b, tid == 0).tiles != 0) continue;
+    if (live_of<S>(a, b, tid == 0).tiles != 0) continue;
     const long long width = static_cast<long long>(a.heads) * a.head_dim;
     for (int h = warp; h < a.heads; h += S::NW)
       for (int d = lane; d < a.head_dim; d += 32) {
@@ -624,7 +709,10 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += live_of<S::TOK>(a, b, false).tiles;
+  for (int b = b0; b < b1; ++b) {
+    const Live v = live_of<S>(a, b, false);
+    if (v.tiles != 0) mine += v.tiles + v.extra;
+  }
   mine *= items;
   long long scan = mine;
 #pragma unroll
@@ -643,16 +731,18 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
     if (w < warp) before += scan_sum[w];
     total += scan_sum[w];
   }
-  // CTAs in use: at least one tile a warp.
-  const int used = static_cast<int>(min(static_cast<long long>(ctas), (total + S::NW - 1) / S::NW));
+  // CTAs in use, and this one's run [x0, x1) of the line.
+  const int used = static_cast<int>(min(static_cast<long long>(ctas), (total + S::MIN_RUN - 1) / S::MIN_RUN));
   if (cta >= used) return;
-  const long long g0 = total * cta / used, g1 = total * (cta + 1) / used;
-  if (before <= g0 && g0 < before + mine) {
+  const long long x0 = static_cast<long long>(divided(total * cta, used));
+  const long long x1 = static_cast<long long>(divided(total * (cta + 1), used));
+  if (before <= x0 && x0 < before + mine) {
     long long base = before;
     int b = b0;
     for (;; ++b) {
-      const long long n = static_cast<long long>(live_of<S::TOK>(a, b, false).tiles) * items;
-      if (g0 < base + n) break;
+      const Live v = live_of<S>(a, b, false);
+      const long long n = v.tiles != 0 ? static_cast<long long>(v.tiles + v.extra) * items : 0;
+      if (x0 < base + n) break;
       base += n;
     }
     found_request = b;
@@ -660,12 +750,12 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   }
   __syncthreads();
 
-  Cursor<S::TOK> at;
-  at.start(a, found_request, found_base, g0, g1);
+  Cursor<S> at;
+  bool run = at.start(a, found_request, found_base, x0, x1);
   Loader<S> loader;
   loader.at = at;
-  loader.tile = warp;
-  loader.more = true;
+  loader.tile = at.first_tile(warp);
+  loader.more = run;
   const uint32_t ring = dg::sm100::smem_addr(smem) + warp * (S::STAGES * S::STAGE);
   uint32_t* mask = masks + warp * S::STAGES;
   loader.prepare(p, warp, lane, items);
@@ -678,9 +768,11 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 
   Warp<S> w;
   int stage = 0;
-  for (bool run = true; run; run = at.advance(a, items)) {
+  for (; run; run = at.advance(a, items)) {
+    int tile = at.first_tile(warp);
+    if (at.solo && tile >= at.count) continue;
     w.begin(p, at.b, at.item, lane);
-    for (int tile = warp; tile < at.count; tile += S::NW) {
+    for (const int step = at.step(); tile < at.count; tile += step) {
       dg::warp::cp_async_wait<S::STAGES - 2>();
       __syncwarp();        // every lane's copies of this stage landed, every lane is done with the one before
       const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
@@ -689,6 +781,11 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       loader.prepare(p, warp, lane, items);
       w.step(p, ring + stage * S::STAGE, mask[stage], lane);
       stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+    }
+
+    if (at.solo) {
+      finish_solo<S>(p, at.b, at.item, w, lane);
+      continue;
     }
 
     // Join the warps.
@@ -774,8 +871,9 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       if (lane == 0) p.share_ml[slot * kMaxRows + row] = make_float2(row_m[i], row_l[i]);
     }
     // The CTAs of the item: those that own its first and its last tile.
-    const int c0 = static_cast<int>(((at.item_g0 + 1) * used - 1) / total);
-    const int c1 = static_cast<int>(((at.item_g0 + n_tiles) * used - 1) / total);
+    const long long first_unit = at.item_x0 + at.live.extra;
+    const int c0 = static_cast<int>(divided((first_unit + 1) * used - 1, total));
+    const int c1 = static_cast<int>(divided((first_unit + n_tiles) * used - 1, total));
     const int n = c1 - c0 + 1;
     __syncthreads();
     if (tid == 0) {

@@ -130,31 +130,33 @@ def test_null_arguments_are_refused():
     assert L.dg_paged_attention(None, None, 0) == BAD
 
 
-def _cut(lens, items, tok, window, ctas, warps):
-    """The attention kernel's cut of a batch: per CTA its shares (request, item,
-    first tile, tiles, line index of the item's first tile)."""
+def _cut(lens, items, tok, window, ctas, warps, extra=8, extra_solo=1, min_run=4):
+    """The attention kernel's cut of a batch: (units, CTAs in use, per CTA its
+    shares (request, item, first tile, tiles, unit of the item's first tile,
+    the item's tiles, one warp's work or not))."""
     line = []
     for b, n in enumerate(lens):
         lo = max(0, n - window) if window else 0
         tiles = (n - 1) // tok + 1 - lo // tok if n else 0
-        line += [(b, i, tiles) for i in range(items)] if tiles else []
-    total = sum(t for _, _, t in line)
-    used = min(ctas, -(-total // warps))
-    shares = [[] for _ in range(used)]
-    at = 0
-    for b, i, tiles in line:
+        line += [(b, i, tiles, extra_solo if tiles <= warps else extra) for i in range(items)] if tiles else []
+    total = sum(t + e for _, _, t, e in line)
+    used = min(ctas, -(-total // min_run))
+    bounds = [total * c // used for c in range(used + 1)]
+    shares, at = [[] for _ in range(used)], 0
+    for b, i, tiles, e in line:
         for c in range(used):
-            g0, g1 = total * c // used, total * (c + 1) // used
-            lo, hi = max(g0, at), min(g1, at + tiles)
-            if lo < hi:
-                shares[c].append((b, i, lo - at, hi - lo, at, tiles))
-        at += tiles
+            lo, hi = max(bounds[c], at), min(bounds[c + 1], at + tiles + e)
+            t0, t1 = max(0, lo - at - e), max(0, min(tiles, hi - at - e))
+            if lo < hi and t0 < t1:
+                solo = tiles <= warps and t1 - t0 == tiles and bounds[c + 1] - bounds[c] >= 2 * (tiles + e)
+                shares[c].append((b, i, t0, t1 - t0, at + e, tiles, solo))
+        at += tiles + e
     return total, used, shares
 
 
 @pytest.mark.parametrize("lens,items,window", [
     ([1], 1, 0), ([2049], 8, 0), ([0, 5, 0, 300, 0], 2, 0), ([17] * 40, 4, 0), ([8191, 1, 33, 0, 4096], 8, 100),
-    ([131072], 1, 0), ([1] * 700, 3, 0), ([1000, 0, 64, 65] * 9, 5, 64)])
+    ([131072], 1, 0), ([1] * 700, 3, 0), ([1000, 0, 64, 65] * 9, 5, 64), ([16] * 3 + [129, 3000], 1, 0)])
 @pytest.mark.parametrize("tok,warps", [(16, 8), (32, 8), (16, 4)])
 def test_attention_shares_meet(lens, items, window, tok, warps):
     """Every tile belongs to one CTA; the CTAs of a shared item are the run
@@ -162,24 +164,30 @@ def test_attention_shares_meet(lens, items, window, tok, warps):
     workspace slots (2c, or 2c + 1 for the share that begins the item), and no
     two shared items have the same ticket c0."""
     total, used, shares = _cut(lens, items, tok, window, 148, warps)
-    assert sum(s[3] for c in shares for s in c) == total
-    assert all(shares), "every CTA in use has work"
-    owners, slots = {}, set()
+    owners, slots, tiles_of = {}, set(), {}
     for c, mine in enumerate(shares):
-        assert len([s for s in mine if s[2] > 0]) <= 1 and all(s[2] == 0 for s in mine[1:])
-        for b, i, t0, count, g0, tiles in mine:
-            c0 = ((g0 + 1) * used - 1) // total
-            c1 = ((g0 + tiles) * used - 1) // total
-            assert c0 <= c <= c1
-            owners.setdefault((b, i), []).append((c, c0, c1))
+        assert all(s[2] == 0 for s in mine[1:])
+        for b, i, t0, count, first, tiles, solo in mine:
+            c0 = ((first + 1) * used - 1) // total
+            c1 = ((first + tiles) * used - 1) // total
+            assert c0 <= c <= c1 and not (solo and c0 != c1)
+            owners.setdefault((b, i), []).append((c, c0, c1, t0, count))
+            tiles_of[b, i] = tiles
             if count < tiles:
                 slot = 2 * c + (1 if t0 == 0 else 0)
                 assert slot not in slots and slot == 2 * c + (1 if c == c0 else 0)
                 slots.add(slot)
+    live = [n for n in lens if n]
+    assert len(owners) == len(live) * items
     tickets = set()
-    for runs in owners.values():
-        c0, c1 = runs[0][1:]
+    for key, runs in owners.items():
+        c0, c1 = runs[0][1:3]
         assert [r[0] for r in runs] == list(range(c0, c1 + 1))
+        at = 0
+        for _, _, _, t0, count in runs:
+            assert t0 == at
+            at += count
+        assert at == tiles_of[key]
         if c1 > c0:
             assert c0 not in tickets
             tickets.add(c0)
