@@ -86,6 +86,7 @@ struct Params {
   int group;               // query heads a kv head
   int groups;              // items a kv head: ceil(group / ROWS)
   int page_shift;          // log2(page_size), -1 if it is no power of two
+  int aligned;             // page_size is a multiple of TOK
   int* tickets;
   float2* share_ml;        // [share][kMaxRows]
   float* share_o;          // [share][kMaxRows][kMaxDim]
@@ -233,43 +234,64 @@ struct Cursor {
 };
 
 // One warp's copies: tile after tile of the CTA's run, ahead of the products.
+// Where page_size is a multiple of TOK (`p.aligned`) a tile lies in one page:
+// one table entry a tile, and a lane's addresses are a line.  Otherwise every
+// lane looks up one token, and its row's address goes round by shuffles.
 template <typename S>
 struct Loader {
+  static constexpr int CH = S::DP * S::ES / 16;     // chunks a row
+  static constexpr int RPI = 32 / CH;               // rows an instruction
+  static constexpr uint32_t kWhole = S::TOK == 32 ? 0xffffffffu : (1u << (S::TOK & 31)) - 1u;
   Cursor<S> at;
   int tile;              // of the share
   bool more;             // a tile is pending
-  // The pending tile: this lane's token.
-  int page, offset, head;
-  bool ok;
+  // The pending tile: its live tokens; page and offset in it of its first
+  // token, or of this lane's.
+  uint32_t bits;
+  int page, offset;
+  // The share's head in the caches; aligned: this lane's row and chunk of it.
+  const char *keys, *values;
 
+  __device__ __forceinline__ void open(const Params& p, int lane) {
+    const dg_attention_args& a = p.a;
+    const int head = p.groups == 1 ? at.item : at.item / p.groups;
+    const int row = p.aligned ? lane / CH : 0, chunk = p.aligned ? lane % CH : 0;
+    keys = static_cast<const char*>(a.k_cache) + (head * a.k_cache_stride[2] + row * a.k_cache_stride[1]) * S::ES +
+           chunk * 16;
+    values = static_cast<const char*>(a.v_cache) + (head * a.v_cache_stride[2] + row * a.v_cache_stride[1]) * S::ES +
+             chunk * 16;
+  }
   __device__ __forceinline__ void look_up(const Params& p, int lane) {
-    const int tok = (at.live.first + at.t0 + tile) * S::TOK + lane;
-    ok = lane < S::TOK && tok >= at.live.lo && tok < at.live.len;
-    page = -1;
-    offset = 0;
-    head = p.groups == 1 ? at.item : at.item / p.groups;
-    if (ok) {
-      const unsigned t = static_cast<unsigned>(tok);
-      unsigned column;
-      if (p.page_shift >= 0) {
-        column = t >> p.page_shift;
-        offset = static_cast<int>(t & ((1u << p.page_shift) - 1u));
-      } else {
-        column = t / static_cast<unsigned>(p.a.page_size);
-        offset = static_cast<int>(t - column * static_cast<unsigned>(p.a.page_size));
-      }
-      page = __ldg(p.a.block_table + at.b * p.a.table_stride + column);
+    const int tok = (at.live.first + at.t0 + tile) * S::TOK;
+    const int from = at.live.lo - tok, to = at.live.len - tok;      // to > 0, from < TOK
+    bits = kWhole;
+    if (to < S::TOK) bits &= (1u << to) - 1u;
+    if (from > 0) bits &= ~((1u << from) - 1u);
+    const unsigned t = static_cast<unsigned>(tok) + (p.aligned ? 0u : static_cast<unsigned>(lane));
+    unsigned column;
+    if (p.page_shift >= 0) {
+      column = t >> p.page_shift;
+      offset = static_cast<int>(t & ((1u << p.page_shift) - 1u));
+    } else {
+      column = t / static_cast<unsigned>(p.a.page_size);
+      offset = static_cast<int>(t - column * static_cast<unsigned>(p.a.page_size));
     }
+    page = -1;
+    if (p.aligned || ((bits >> (lane % S::TOK)) & 1u & (lane < S::TOK)) != 0u)
+      page = __ldg(p.a.block_table + at.b * p.a.table_stride + column);
   }
   // Moves to the warp's next tile, through the shares that have none for it.
   __device__ __forceinline__ void prepare(const Params& p, int warp, int lane, int items) {
     if (!more) return;
-    while (tile >= at.count) {
-      if (!at.advance(p.a, items)) {
-        more = false;
-        return;
-      }
-      tile = at.first_tile(warp);
+    if (tile >= at.count) {
+      do {
+        if (!at.advance(p.a, items)) {
+          more = false;
+          return;
+        }
+        tile = at.first_tile(warp);
+      } while (tile >= at.count);
+      open(p, lane);
     }
     look_up(p, lane);
     tile += at.step();
@@ -278,33 +300,64 @@ struct Loader {
   __device__ __forceinline__ void issue(const Params& p, uint32_t stage, uint32_t* mask, int lane) const {
     if (!more) return;
     const dg_attention_args& a = p.a;
-    bool good = ok;
-    if (ok && (page < 0 || page >= a.num_pages)) {
-      report(a.status, DG_ERR_PAGE);
-      good = false;
-    }
-    const uint32_t live = __ballot_sync(0xffffffffu, good);
-    if (lane == 0) *mask = live;
-    long long k_at = 0, v_at = 0;
-    if (good) {
-      k_at = page * a.k_cache_stride[0] + offset * a.k_cache_stride[1] + head * a.k_cache_stride[2];
-      v_at = page * a.v_cache_stride[0] + offset * a.v_cache_stride[1] + head * a.v_cache_stride[2];
-    }
-    constexpr int CH = S::DP * S::ES / 16;      // chunks a row
-    constexpr int RPI = 32 / CH;                // rows an instruction
     const int chunk = lane % CH;
     const bool wanted = chunk * 16 < a.head_dim * S::ES;
+    // Row i * RPI + lane / CH: its swizzle is the lane's and the row step's.
+    const uint32_t dst = stage + (lane / CH) * S::PITCH + S::swizzled(lane / CH, chunk) * 16;
+    const bool good = page >= 0 && page < a.num_pages;
+    if (p.aligned) {
+      if (!good && lane == 0) report(a.status, DG_ERR_PAGE);
+      const uint32_t live = good ? bits : 0u;
+      if (lane == 0) *mask = live;
+      const char* k = keys + (page * a.k_cache_stride[0] + offset * a.k_cache_stride[1]) * S::ES;
+      const char* v = values + (page * a.v_cache_stride[0] + offset * a.v_cache_stride[1]) * S::ES;
+      const long long k_step = a.k_cache_stride[1] * (RPI * S::ES), v_step = a.v_cache_stride[1] * (RPI * S::ES);
+      if (live == kWhole) {
+#pragma unroll
+        for (int i = 0; i < S::TOK / RPI; ++i, k += k_step, v += v_step) {
+          const uint32_t to = (dst ^ (S::swizzled(i * RPI, 0) * 16)) + i * RPI * S::PITCH;
+          if (wanted) {
+            dg::warp::cp_async16(to, k);
+            dg::warp::cp_async16(to + S::KV_BYTES, v);
+          }
+        }
+      } else {
+        if (!good) {         // nothing is read, but the addresses are still some
+          k = static_cast<const char*>(a.k_cache);
+          v = static_cast<const char*>(a.v_cache);
+        }
+        const long long ks = good ? k_step : 0, vs = good ? v_step : 0;
+#pragma unroll
+        for (int i = 0; i < S::TOK / RPI; ++i, k += ks, v += vs) {
+          const uint32_t to = (dst ^ (S::swizzled(i * RPI, 0) * 16)) + i * RPI * S::PITCH;
+          const uint32_t bytes = (live >> (i * RPI + lane / CH)) & 1u ? 16u : 0u;
+          if (wanted) {
+            dg::warp::cp_async16(to, k, bytes);
+            dg::warp::cp_async16(to + S::KV_BYTES, v, bytes);
+          }
+        }
+      }
+      return;
+    }
+    const bool seen = lane < S::TOK && ((bits >> (lane % S::TOK)) & 1u) != 0u;
+    if (seen && !good) report(a.status, DG_ERR_PAGE);
+    const uint32_t live = __ballot_sync(0xffffffffu, seen && good);
+    if (lane == 0) *mask = live;
+    long long k_at = 0, v_at = 0;
+    if (seen && good) {
+      k_at = (page * a.k_cache_stride[0] + offset * a.k_cache_stride[1]) * S::ES;
+      v_at = (page * a.v_cache_stride[0] + offset * a.v_cache_stride[1]) * S::ES;
+    }
 #pragma unroll
     for (int i = 0; i < S::TOK / RPI; ++i) {
       const int r = i * RPI + lane / CH;
       const long long kr = __shfl_sync(0xffffffffu, k_at, r);
       const long long vr = __shfl_sync(0xffffffffu, v_at, r);
       const uint32_t bytes = (live >> r) & 1u ? 16u : 0u;
-      const uint32_t dst = stage + r * S::PITCH + S::swizzled(r, chunk) * 16;
+      const uint32_t to = (dst ^ (S::swizzled(i * RPI, 0) * 16)) + i * RPI * S::PITCH;
       if (wanted) {
-        dg::warp::cp_async16(dst, static_cast<const char*>(a.k_cache) + kr * S::ES + (bytes ? chunk * 16 : 0), bytes);
-        dg::warp::cp_async16(dst + S::KV_BYTES,
-                             static_cast<const char*>(a.v_cache) + vr * S::ES + (bytes ? chunk * 16 : 0), bytes);
+        dg::warp::cp_async16(to, keys + kr + (bytes ? chunk * 16 : 0), bytes);
+        dg::warp::cp_async16(to + S::KV_BYTES, values + vr + (bytes ? chunk * 16 : 0), bytes);
       }
     }
   }
@@ -408,8 +461,9 @@ struct Warp {
 
     if constexpr (!S::kE4m3) {
       // Matrices: tokens 0-7 x (values 0-7, 8-15), tokens 8-15 x the same.
-      const int row = (lane & 7) + (lane >> 4) * 8, side = (lane >> 3) & 1;
-      const uint32_t at = keys + row * S::PITCH;
+      // Chunk 2 ks + side of the row; stages are aligned to 128 bytes, so that
+      // the step's part of the chunk goes in by exclusive or and offset.
+      const uint32_t at = keys + ((lane & 7) + (lane >> 4) * 8) * S::PITCH + S::swizzled(lane, (lane >> 3) & 1) * 16;
 #pragma unroll
       for (int ks = 0; ks < S::KS; ++ks) {
         uint32_t x[4];
@@ -417,7 +471,7 @@ struct Warp {
 #pragma unroll
         for (int t = 0; t < S::NT; t += 2) {
           uint32_t k[4];
-          dg::warp::ldmatrix_x4(k, at + t * 8 * S::PITCH + S::swizzled(lane, ks * 2 + side) * 16);
+          dg::warp::ldmatrix_x4(k, (at ^ (ks * 32 & 127)) + (ks * 32 & ~127) + t * 8 * S::PITCH);
           S::MM::mma(s[t], x, k[0], k[1]);
           S::MM::mma(s[t + 1], x, k[2], k[3]);
         }
@@ -514,11 +568,11 @@ struct Warp {
         }
       }
       if constexpr (!S::kE4m3) {
-        const uint32_t at = values + (kk * 16 + (lane & 15)) * S::PITCH;
+        const uint32_t at = values + (lane & 15) * S::PITCH + S::swizzled(lane, lane >> 4) * 16;
 #pragma unroll
         for (int t = 0; t < S::OT; t += 2) {
           uint32_t v[4];
-          dg::warp::ldmatrix_x4_trans(v, at + S::swizzled(lane, t + (lane >> 4)) * 16);
+          dg::warp::ldmatrix_x4_trans(v, (at ^ (t * 16 & 127)) + (t * 16 & ~127) + kk * 16 * S::PITCH);
           S::MM::mma(o[t], x, v[0], v[1]);
           S::MM::mma(o[t + 1], x, v[2], v[3]);
           if constexpr (R == 2) {
@@ -756,6 +810,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   loader.at = at;
   loader.tile = at.first_tile(warp);
   loader.more = run;
+  if (run) loader.open(p, lane);
   const uint32_t ring = dg::sm100::smem_addr(smem) + warp * (S::STAGES * S::STAGE);
   uint32_t* mask = masks + warp * S::STAGES;
   loader.prepare(p, warp, lane, items);
@@ -932,13 +987,13 @@ using Kernel = void (*)(const Params);
 struct Entry {
   Kernel fn;
   size_t smem;
-  int threads, rows;
+  int threads, rows, tok;
   std::atomic<unsigned long long> ready;    // per device: shared memory limit raised
 };
 
 template <typename S>
 Entry& entry() {
-  static Entry e{attention_kernel<S>, S::SMEM, S::NW * 32, S::ROWS, {0}};
+  static Entry e{attention_kernel<S>, S::SMEM, S::NW * 32, S::ROWS, S::TOK, {0}};
   return e;
 }
 
@@ -1000,6 +1055,7 @@ int dg_paged_attention(const dg_attention_args* args, void* stream, int pdl_attr
     p.page_shift = 0;
     while ((1 << p.page_shift) < p.a.page_size) ++p.page_shift;
   }
+  p.aligned = p.a.page_size % e.tok == 0 ? 1 : 0;
   unsigned char* ws = static_cast<unsigned char*>(p.a.workspace);
   p.tickets = reinterpret_cast<int*>(ws);
   p.share_ml = reinterpret_cast<float2*>(ws + kTicketBytes);
