@@ -42,8 +42,7 @@
 // consecutive bytes a lane: no 8-bit transposition.  q is scaled by a power
 // of two per head to fit fp16's range, exactly undone in fp32.
 //
-// Join.  The warps' (m, l, o) are joined in shared memory, 32 columns at a
-// time, in warp order.  A share of an item goes to the workspace; the last
+// Join.  The warps' (m, l, o) are joined in shared memory, in warp order.  A share of an item goes to the workspace; the last
 // of the item's CTAs to arrive (a ticket) joins the shares in CTA order.
 // No CTA waits for another.
 
@@ -107,9 +106,8 @@ struct Shape {
   static constexpr int KV_BYTES = TOK * PITCH;                   // a stage's keys; its values follow
   static constexpr int STAGE = 2 * KV_BYTES;
   static constexpr int RING = NW * STAGES * STAGE;
-  static constexpr int JOIN_ROW = 40;                            // 32 columns, padded against bank conflicts
-  static constexpr int JOIN_BUFS = ROWS_ == 8 ? 2 : 1;
-  static constexpr int JOIN = NW * ROWS_ * JOIN_ROW;             // floats a buffer
+  static constexpr int JOIN = 8192;                              // floats of the join's buffer (32 KiB)
+  static constexpr int JOIN_COLS = JOIN / (NW * ROWS_) < DP_ ? JOIN / (NW * ROWS_) : DP_;   // columns a round
   static constexpr int SOLO = NW;                                // tiles of an item that one warp does alone
   static constexpr int EXTRA_SOLO = 1, EXTRA = 8;                // an item's cost in tiles, beyond its tiles
   static constexpr int MIN_RUN = 4;                              // units a CTA takes at least
@@ -121,10 +119,10 @@ struct Shape {
   // 2^kBias is the probability of the maximum: fp16's subnormals start at
   // 2^-14, so its probabilities are lifted out of them.
   static constexpr float kBias = sizeof(MM_) != 0 && __is_same(MM_, Fp16) ? 10.0f : 0.0f;
-  static constexpr size_t SMEM = RING + sizeof(float) * (JOIN_BUFS * JOIN + 2 * NW * ROWS_) +
+  static constexpr size_t SMEM = RING + sizeof(float) * (JOIN + 2 * NW * ROWS_) +
                                  sizeof(uint32_t) * NW * STAGES;
   static_assert(ROWS_ % NW == 0 && SMEM <= 227 * 1024 - 1024, "shared memory");
-  static_assert(kMaxCtas * ROWS_ <= JOIN_BUFS * JOIN, "join factors fit the join buffers");
+  static_assert(kMaxCtas * ROWS_ <= JOIN, "join factors fit the join buffers");
 
   // Output column of position `n` of output tile `t` (see the e4m3 fragments).
   static __device__ __forceinline__ int column(int t, int n) {
@@ -375,16 +373,17 @@ struct Warp {
   uint32_t q[S::KS][2 * R];                          // [step][first half's rows, second half's rows]
   float o[S::OT][4];
   float m[R], l[R];
-  float factor[R];                                   // score -> exponent of 2 (or -> argument of tanh)
+  float factor[R];                                   // score -> exponent of 2 (capped: of the tanh's exponential)
 
-  __device__ __forceinline__ void begin(const Params& p, int b, int item, int lane) {
+  // Loads an item's q as it lies in memory; nothing waits for it before
+  // begin().
+  __device__ __forceinline__ void fetch(const Params& p, int b, int item, int lane) {
     const dg_attention_args& a = p.a;
     const int head = p.groups == 1 ? item : item / p.groups;
-    const int part = item - head * p.groups;
     const int quad = lane & 3;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      const int row = part * S::ROWS + (lane >> 2) + 8 * r;
+      const int row = (item - head * p.groups) * S::ROWS + (lane >> 2) + 8 * r;
       const uint16_t* src = static_cast<const uint16_t*>(a.q) + b * a.q_stride[0] +
                             (static_cast<long long>(head) * p.group + row) * a.q_stride[1];
       const bool real = row < p.group;
@@ -398,6 +397,13 @@ struct Warp {
           q[ks][h * R + r] = real && d < a.head_dim ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
         }
       }
+    }
+  }
+
+  __device__ __forceinline__ void begin(const Params& p, int item) {
+    const dg_attention_args& a = p.a;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
       float f = a.scale;
       if constexpr (S::kE4m3) {
         float top = 0.0f;
@@ -423,9 +429,9 @@ struct Warp {
             q[ks][h * R + r] = Fp16::pack(v.x * down, v.y * down);
           }
         f *= up;
-        if (a.k_scale != nullptr) f *= a.k_scale[head];
+        if (a.k_scale != nullptr) f *= a.k_scale[p.groups == 1 ? item : item / p.groups];
       }
-      factor[r] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
+      factor[r] = a.softcap > 0.0f ? 2.0f * kLog2e * (f / a.softcap) : f * kLog2e;
       m[r] = kNegInf;
       l[r] = 0.0f;
     }
@@ -488,7 +494,7 @@ struct Warp {
           for (int i = 0; i < 4; ++i) {
             uint32_t x[4];
             a_of(blk * 4 + i, x);
-            S::MM::mma(s[t], x, dg::warp::e4m3x2_to_f16x2(w[i]), dg::warp::e4m3x2_to_f16x2(w[i] >> 16));
+            S::MM::mma(s[t], x, dg::warp::e4m3_low(w[i]), dg::warp::e4m3_high(w[i]));
           }
         }
       }
@@ -508,7 +514,9 @@ struct Warp {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float x = s[t][2 * r + i] * factor[r];
-          if (capped) x = tanhf(x) * cap;
+          // tanh(x) = 1 - 2 / (e^(2x) + 1): off by about 2^-22, as the score that
+          // it is a part of (cap = softcap * log2 e, factor has 2 log2 e).
+          if (capped) x = cap - 2.0f * cap * dg::warp::rcp_approx(dg::warp::exp2_approx(x) + 1.0f);
           if (!whole && ((live >> (t * 8 + quad * 2 + i)) & 1u) == 0u) x = kNegInf;
           s[t][2 * r + i] = x;
           top = fmaxf(top, x);
@@ -599,8 +607,8 @@ struct Warp {
             const uint32_t b1 = __byte_perm(w < 2 ? v[2].x : v[2].y, w < 2 ? v[3].x : v[3].y, sel);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const uint32_t f0 = dg::warp::e4m3x2_to_f16x2(b0 >> (16 * c));
-              const uint32_t f1 = dg::warp::e4m3x2_to_f16x2(b1 >> (16 * c));
+              const uint32_t f0 = c ? dg::warp::e4m3_high(b0) : dg::warp::e4m3_low(b0);
+              const uint32_t f1 = c ? dg::warp::e4m3_high(b1) : dg::warp::e4m3_low(b1);
               S::MM::mma(o[j * 8 + w * 2 + c], x, f0, f1);
               if constexpr (R == 2) S::MM::mma(o[j * 8 + w * 2 + c], y, f0, f1);
             }
@@ -726,8 +734,8 @@ __device__ __forceinline__ void finish_solo(const Params& p, int b, int item, co
 template <typename S>
 __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  float* join = reinterpret_cast<float*>(smem + S::RING);               // [JOIN_BUFS][NW][ROWS][JOIN_ROW]
-  float* warp_m = join + S::JOIN_BUFS * S::JOIN;                        // [NW][ROWS]
+  float* join = reinterpret_cast<float*>(smem + S::RING);               // [NW][ROWS][JOIN_COLS]
+  float* warp_m = join + S::JOIN;                                       // [NW][ROWS]
   float* warp_l = warp_m + S::NW * S::ROWS;
   uint32_t* masks = reinterpret_cast<uint32_t*>(warp_l + S::NW * S::ROWS);   // [NW][STAGES]
   __shared__ long long scan_sum[S::NW];
@@ -823,23 +831,31 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 
   Warp<S> w;
   int stage = 0;
-  for (; run; run = at.advance(a, items)) {
-    int tile = at.first_tile(warp);
-    if (at.solo && tile >= at.count) continue;
-    w.begin(p, at.b, at.item, lane);
-    for (const int step = at.step(); tile < at.count; tile += step) {
-      dg::warp::cp_async_wait<S::STAGES - 2>();
-      __syncwarp();        // every lane's copies of this stage landed, every lane is done with the one before
-      const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
-      loader.issue(p, ring + ahead * S::STAGE, mask + ahead, lane);
-      dg::warp::cp_async_commit();
-      loader.prepare(p, warp, lane, items);
-      w.step(p, ring + stage * S::STAGE, mask[stage], lane);
-      stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+  bool mine_too = run && (!at.solo || at.first_tile(warp) == 0);
+  if (mine_too) w.fetch(p, at.b, at.item, lane);
+  while (run) {
+    const Cursor<S> share = at;
+    const bool work = mine_too;
+    if (work) {
+      w.begin(p, share.item);
+      const int step = share.step();
+      for (int tile = share.first_tile(warp); tile < share.count; tile += step) {
+        dg::warp::cp_async_wait<S::STAGES - 2>();
+        __syncwarp();      // every lane's copies of this stage landed, every lane is done with the one before
+        const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
+        loader.issue(p, ring + ahead * S::STAGE, mask + ahead, lane);
+        dg::warp::cp_async_commit();
+        loader.prepare(p, warp, lane, items);
+        w.step(p, ring + stage * S::STAGE, mask[stage], lane);
+        stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+      }
     }
-
-    if (at.solo) {
-      finish_solo<S>(p, at.b, at.item, w, lane);
+    // The next share's q is on its way during the join.
+    run = at.advance(a, items);
+    mine_too = run && (!at.solo || at.first_tile(warp) == 0);
+    if (mine_too) w.fetch(p, at.b, at.item, lane);
+    if (share.solo) {
+      if (work) finish_solo<S>(p, share.b, share.item, w, lane);
       continue;
     }
 
@@ -879,18 +895,21 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       row_m[i] = top;
       row_l[i] = l;
     }
+    // Column x of row r stands at x ^ 8 (r % 4): neither the writes (4 rows, 8
+    // columns each) nor the reads (32 columns of a row) meet in a bank.
+    constexpr int ROUND_CHUNKS = S::JOIN_COLS / 32;
 #pragma unroll
-    for (int c = 0; c < S::CHUNKS; ++c) {
-      float* buf = join + (S::JOIN_BUFS == 2 ? (c & 1) * S::JOIN : 0);
+    for (int c0 = 0; c0 < S::CHUNKS; c0 += ROUND_CHUNKS) {
+      if (c0 != 0) __syncthreads();
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const float(&o)[4] = w.o[c * 4 + t];
-        float* dst = buf + (warp * S::ROWS + g) * S::JOIN_ROW + t * 8 + quad * 2;
+      for (int t = 0; t < ROUND_CHUNKS * 4; ++t) {
+        const float(&o)[4] = w.o[c0 * 4 + t];
+        float* dst = join + (warp * S::ROWS + g) * S::JOIN_COLS + ((t * 8 + quad * 2) ^ ((g & 3) * 8));
         if constexpr (S::ROWS == 8) {
           *reinterpret_cast<float2*>(dst) = make_float2((o[0] + o[2]) * mine_by[0], (o[1] + o[3]) * mine_by[0]);
         } else {
           *reinterpret_cast<float2*>(dst) = make_float2(o[0] * mine_by[0], o[1] * mine_by[0]);
-          *reinterpret_cast<float2*>(dst + 8 * S::JOIN_ROW) =
+          *reinterpret_cast<float2*>(dst + 8 * S::JOIN_COLS) =
               make_float2(o[2] * mine_by[Warp<S>::R - 1], o[3] * mine_by[Warp<S>::R - 1]);
         }
       }
@@ -898,25 +917,28 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < S::RPT; ++i) {
         const int row = warp + i * S::NW;
-        float v = 0.0f;
 #pragma unroll
-        for (int u = 0; u < S::NW; ++u) v += buf[(u * S::ROWS + row) * S::JOIN_ROW + lane];
-        sum[i][c] = v;
+        for (int c = 0; c < ROUND_CHUNKS; ++c) {
+          float v = 0.0f;
+#pragma unroll
+          for (int u = 0; u < S::NW; ++u)
+            v += join[(u * S::ROWS + row) * S::JOIN_COLS + ((c * 32 + lane) ^ ((row & 3) * 8))];
+          sum[i][c0 + c] = v;
+        }
       }
-      if (S::JOIN_BUFS == 1) __syncthreads();
     }
 
-    const int n_tiles = at.live.tiles;
-    if (at.count == n_tiles) {              // the whole item
+    const int n_tiles = share.live.tiles;
+    if (share.count == n_tiles) {              // the whole item
 #pragma unroll
       for (int i = 0; i < S::RPT; ++i)
-        finish_row<S>(p, at.b, at.item, warp + i * S::NW, sum[i], row_m[i], row_l[i], lane);
+        finish_row<S>(p, share.b, share.item, warp + i * S::NW, sum[i], row_m[i], row_l[i], lane);
       continue;
     }
 
     // A share: to the workspace, slot 2c for an item that began in an earlier
     // CTA, 2c + 1 for one that begins here.
-    const size_t slot = 2 * static_cast<size_t>(cta) + (at.t0 == 0 ? 1 : 0);
+    const size_t slot = 2 * static_cast<size_t>(cta) + (share.t0 == 0 ? 1 : 0);
 #pragma unroll
     for (int i = 0; i < S::RPT; ++i) {
       const int row = warp + i * S::NW;
@@ -926,7 +948,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       if (lane == 0) p.share_ml[slot * kMaxRows + row] = make_float2(row_m[i], row_l[i]);
     }
     // The CTAs of the item: those that own its first and its last tile.
-    const long long first_unit = at.item_x0 + at.live.extra;
+    const long long first_unit = share.item_x0 + share.live.extra;
     const int c0 = static_cast<int>(divided((first_unit + 1) * used - 1, total));
     const int c1 = static_cast<int>(divided((first_unit + n_tiles) * used - 1, total));
     const int n = c1 - c0 + 1;
@@ -975,7 +997,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 #pragma unroll
         for (int k = 0; k < S::CHUNKS; ++k) v[k] += f * __ldcg(src + k * 32);
       }
-      finish_row<S>(p, at.b, at.item, row, v, top, l, lane);
+      finish_row<S>(p, share.b, share.item, row, v, top, l, lane);
     }
     __syncthreads();                        // the join buffers and is_last are free again
   }

@@ -78,6 +78,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
+// 1 / x to 1 ulp; 0 for infinity.
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t as_u32(__nv_bfloat162 v) { return *reinterpret_cast<uint32_t*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 
@@ -113,11 +120,16 @@ struct Fp16 {
   }
 };
 
-// Two e4m3 values (low 16 bits, in order) as a pair of fp16 values: exact,
-// NaN stays NaN.
-__device__ __forceinline__ uint32_t e4m3x2_to_f16x2(uint32_t two) {
+// The two e4m3 values in the low / high half of a word as a pair of fp16
+// values: exact, NaN stays NaN.
+__device__ __forceinline__ uint32_t e4m3_low(uint32_t four) {
   uint32_t r;
-  asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two));
+  asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(four));
+  return r;
+}
+__device__ __forceinline__ uint32_t e4m3_high(uint32_t four) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 t, u;\n\tmov.b32 {t, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, u;\n\t}" : "=r"(r) : "r"(four));
   return r;
 }
 
