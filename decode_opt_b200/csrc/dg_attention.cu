@@ -99,29 +99,30 @@ struct Shape {
   static constexpr bool kE4m3 = E4M3_;
   static constexpr int DP = DP_, ROWS = ROWS_;
   static constexpr int ES = E4M3_ ? 1 : 2;
-  static constexpr int NW = DP_ == 256 ? 4 : 8;                  // warps
+  static constexpr int NW = DP_ == 64 ? 12 : DP_ == 128 ? 8 : 4; // warps
   static constexpr int TOK = E4M3_ || DP_ == 64 ? 32 : 16;       // tokens a stage
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = DP_ == 64 ? 2 : 3;
   static constexpr int PITCH = DP_ * ES;                         // bytes a row
   static constexpr int KV_BYTES = TOK * PITCH;                   // a stage's keys; its values follow
   static constexpr int STAGE = 2 * KV_BYTES;
   static constexpr int RING = NW * STAGES * STAGE;
   static constexpr int JOIN = 8192;                              // floats of the join's buffer (32 KiB)
-  static constexpr int JOIN_COLS = JOIN / (NW * ROWS_) < DP_ ? JOIN / (NW * ROWS_) : DP_;   // columns a round
-  static constexpr int SOLO = NW;                                // tiles of an item that one warp does alone
+  static constexpr int JOIN_COLS =                               // columns a round: a power of two from 32
+      NW * ROWS_ * DP_ <= JOIN ? DP_ : NW * ROWS_ * 128 <= JOIN ? 128 : NW * ROWS_ * 64 <= JOIN ? 64 : 32;
+  static constexpr int SOLO = 8;                                 // tiles of an item that one warp does alone
   static constexpr int EXTRA_SOLO = 1, EXTRA = 8;                // an item's cost in tiles, beyond its tiles
   static constexpr int MIN_RUN = 4;                              // units a CTA takes at least
   static constexpr int NT = TOK / 8;                             // score tiles of 8 tokens
   static constexpr int KS = DP_ / 16;                            // inner steps of Q K^T
   static constexpr int OT = DP_ / 8;                             // output tiles of 8 columns
   static constexpr int CHUNKS = DP_ / 32;                        // of the joins
-  static constexpr int RPT = ROWS_ / NW;                         // rows a warp finishes
+  static constexpr int RPT = (ROWS_ + NW - 1) / NW;              // rows a warp finishes: warp, warp + NW, ...
   // 2^kBias is the probability of the maximum: fp16's subnormals start at
   // 2^-14, so its probabilities are lifted out of them.
   static constexpr float kBias = sizeof(MM_) != 0 && __is_same(MM_, Fp16) ? 10.0f : 0.0f;
   static constexpr size_t SMEM = RING + sizeof(float) * (JOIN + 2 * NW * ROWS_) +
                                  sizeof(uint32_t) * NW * STAGES;
-  static_assert(ROWS_ % NW == 0 && SMEM <= 227 * 1024 - 1024, "shared memory");
+  static_assert(NW * ROWS_ * JOIN_COLS <= JOIN && SMEM <= 227 * 1024 - 1024, "shared memory");
   static_assert(kMaxCtas * ROWS_ <= JOIN, "join factors fit the join buffers");
 
   // Output column of position `n` of output tile `t` (see the e4m3 fragments).
@@ -148,78 +149,82 @@ __device__ __forceinline__ unsigned long long divided(unsigned long long a, unsi
   return a / b;
 }
 
-// A request's live tokens as tiles, and what one of its items costs beyond
-// them.
-struct Live {
-  int lo, len;    // live tokens [lo, len)
-  int first;      // first tile
-  int tiles;      // tiles, 0 if nothing is live
-  int extra;      // units of the line before the item's first tile
-};
-
+// The live tokens [first_live, len) of a request as tiles.
+__device__ __forceinline__ int first_live(const dg_attention_args& a, int len) {
+  return a.window > 0 && len > a.window ? len - a.window : 0;
+}
 template <typename S>
-__device__ __forceinline__ Live live_of(const dg_attention_args& a, int b, bool tell) {
-  Live v;
-  int len = a.seq_lens[b];
+__device__ __forceinline__ int tiles_of(const dg_attention_args& a, int len) {
+  return len > 0 ? (len - 1) / S::TOK + 1 - first_live(a, len) / S::TOK : 0;
+}
+// Units of the line before an item's first tile: what the item costs beyond
+// its tiles.
+template <typename S>
+__device__ __forceinline__ int extra_of(int tiles) {
+  return tiles <= S::SOLO ? S::EXTRA_SOLO : S::EXTRA;
+}
+__device__ __forceinline__ int length_of(const dg_attention_args& a, int b, bool tell) {
+  const int len = a.seq_lens[b];
   const long long most = static_cast<long long>(a.table_width) * a.page_size;
-  if (len < 0 || len > most) {
-    if (tell) report(a.status, DG_ERR_SEQ_LEN);
-    len = len < 0 ? 0 : static_cast<int>(most);
-  }
-  v.len = len;
-  v.lo = a.window > 0 && len > a.window ? len - a.window : 0;
-  v.first = v.lo / S::TOK;
-  v.tiles = len > 0 ? (len - 1) / S::TOK + 1 - v.first : 0;
-  v.extra = v.tiles <= S::SOLO ? S::EXTRA_SOLO : S::EXTRA;
-  return v;
+  if (len >= 0 && len <= most) return len;
+  if (tell) report(a.status, DG_ERR_SEQ_LEN);
+  return len < 0 ? 0 : static_cast<int>(most);
+}
+// The units of all of a request's items.
+template <typename S>
+__device__ __forceinline__ long long units_of(const dg_attention_args& a, int b, int items) {
+  const int tiles = tiles_of<S>(a, length_of(a, b, false));
+  return tiles != 0 ? static_cast<long long>(tiles + extra_of<S>(tiles)) * items : 0;
 }
 
-// A place in a CTA's run [x, x1) of the line: one item's share.
+// A place in a CTA's run of the line, in units from the run's beginning (a
+// run of 2^31 units would be 10^13 bytes): one item's share.
 template <typename S>
 struct Cursor {
-  long long x1;          // end of the CTA's run
-  long long item_x0;     // the item's first unit
+  int run;               // the run's units
+  int x;                 // the item's first unit (below 0: in an earlier CTA's run)
   int b, item;           // request, item of the request
+  int len, tiles;        // the request's length, an item's tiles
   int t0, count;         // the share: tiles [t0, t0 + count) of the item
   int turn;              // solo shares before this one
   bool solo;             // one warp's work (turn % NW) instead of the CTA's
-  long long run;         // the run's units
-  Live live;
 
   // The share [t0, ...) of the item; false if the run ends before it.
   __device__ __forceinline__ bool settle() {
-    const long long end = x1 - item_x0 - live.extra;
-    count = static_cast<int>(min(static_cast<long long>(live.tiles), end)) - t0;
+    const int extra = extra_of<S>(tiles);
+    count = min(tiles, run - x - extra) - t0;
     // One warp takes as many steps as the item has tiles, but several items go
     // side by side: worth it where the run holds more than the one.
-    solo = live.tiles <= S::SOLO && count == live.tiles && run >= 2 * (live.tiles + live.extra);
+    solo = tiles <= S::SOLO && count == tiles && run >= 2 * (tiles + extra);
     return count > 0;
   }
+  // At the unit `from` of the line; request `request` begins at unit `base`.
   __device__ __forceinline__ bool start(const dg_attention_args& a, int request, long long base, long long from,
                                         long long to) {
     b = request;
-    x1 = to;
-    run = to - from;
+    run = static_cast<int>(to - from);
     turn = 0;
-    live = live_of<S>(a, b, false);
-    const int units = live.tiles + live.extra;
+    len = length_of(a, b, false);
+    tiles = tiles_of<S>(a, len);
+    const int units = tiles + extra_of<S>(tiles);
     const unsigned long long off = static_cast<unsigned long long>(from - base);
     item = static_cast<int>(divided(off, static_cast<unsigned long long>(units)));
-    item_x0 = base + static_cast<long long>(item) * units;
-    t0 = max(0, static_cast<int>(from - item_x0) - live.extra);
+    x = -static_cast<int>(off - static_cast<unsigned long long>(item) * units);
+    t0 = max(0, -x - extra_of<S>(tiles));
     return settle();
   }
   // To the next share; false at the end of the run.
   __device__ __forceinline__ bool advance(const dg_attention_args& a, int items) {
-    item_x0 += live.tiles + live.extra;
-    if (item_x0 >= x1) return false;
+    x += tiles + extra_of<S>(tiles);
+    if (x >= run) return false;
     if (solo) ++turn;
     if (++item == items) {
       item = 0;
       do {
-        ++b;             // item_x0 < x1: a later request has tiles
-        live = live_of<S>(a, b, false);
-      } while (live.tiles == 0);
+        ++b;             // x < run: a later request has tiles
+        len = length_of(a, b, false);
+        tiles = tiles_of<S>(a, len);
+      } while (tiles == 0);
     }
     t0 = 0;
     return settle();
@@ -260,8 +265,9 @@ struct Loader {
              chunk * 16;
   }
   __device__ __forceinline__ void look_up(const Params& p, int lane) {
-    const int tok = (at.live.first + at.t0 + tile) * S::TOK;
-    const int from = at.live.lo - tok, to = at.live.len - tok;      // to > 0, from < TOK
+    const int lo = first_live(p.a, at.len);
+    const int tok = (lo / S::TOK + at.t0 + tile) * S::TOK;
+    const int from = lo - tok, to = at.len - tok;      // to > 0, from < TOK
     bits = kWhole;
     if (to < S::TOK) bits &= (1u << to) - 1u;
     if (from > 0) bits &= ~((1u << from) - 1u);
@@ -483,12 +489,13 @@ struct Warp {
         }
       }
     } else {
+      const uint32_t at = keys + g * S::PITCH + S::swizzled(g, quad) * 16;    // chunk 4 blk + quad, as above
 #pragma unroll
       for (int blk = 0; blk < S::KS / 4; ++blk) {
 #pragma unroll
         for (int t = 0; t < S::NT; ++t) {
-          const int r = t * 8 + g;
-          const uint4 k = dg::warp::ld_shared_v4(keys + r * S::PITCH + S::swizzled(r, blk * 4 + quad) * 16);
+          const uint4 k =
+              dg::warp::ld_shared_v4((at ^ (blk * 64 & 127)) + (blk * 64 & ~127) + t * 8 * S::PITCH);
           const uint32_t w[4] = {k.x, k.y, k.z, k.w};
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -503,7 +510,26 @@ struct Warp {
     // Exponents, masked; the running maximum and sum.
     const bool capped = p.a.softcap > 0.0f;
     const float cap = p.a.softcap * kLog2e;
-    const bool whole = live == (S::TOK == 32 ? 0xffffffffu : (1u << (S::TOK & 31)) - 1u);
+#pragma unroll
+    for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2 * R; ++i) s[t][i] *= factor[i >> 1];
+    if (capped) {
+      // tanh(x) = 1 - 2 / (e^(2x) + 1): off by about 2^-22, as the score that
+      // it is a part of (cap = softcap * log2 e, factor has 2 log2 e).
+#pragma unroll
+      for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i)
+          s[t][i] = cap - 2.0f * cap * dg::warp::rcp_approx(dg::warp::exp2_approx(s[t][i]) + 1.0f);
+    }
+    if (live != Loader<S>::kWhole) {
+#pragma unroll
+      for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i)
+          if (((live >> (t * 8 + quad * 2 + (i & 1))) & 1u) == 0u) s[t][i] = kNegInf;
+    }
     float alpha[R];
     bool moved = false;
 #pragma unroll
@@ -512,15 +538,7 @@ struct Warp {
 #pragma unroll
       for (int t = 0; t < S::NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float x = s[t][2 * r + i] * factor[r];
-          // tanh(x) = 1 - 2 / (e^(2x) + 1): off by about 2^-22, as the score that
-          // it is a part of (cap = softcap * log2 e, factor has 2 log2 e).
-          if (capped) x = cap - 2.0f * cap * dg::warp::rcp_approx(dg::warp::exp2_approx(x) + 1.0f);
-          if (!whole && ((live >> (t * 8 + quad * 2 + i)) & 1u) == 0u) x = kNegInf;
-          s[t][2 * r + i] = x;
-          top = fmaxf(top, x);
-        }
+        for (int i = 0; i < 2; ++i) top = fmaxf(top, s[t][2 * r + i]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       moved = moved || top > m[r];
@@ -591,13 +609,15 @@ struct Warp {
       } else {
         // A lane holds 8 consecutive columns 64 j + 8 g of its tokens 2 quad,
         // + 1, + 8, + 9: position g of the 8 output tiles of block j.
+        const uint32_t at = values + quad * 2 * S::PITCH + S::swizzled(quad * 2, g >> 1) * 16 + (g & 1) * 8;
 #pragma unroll
         for (int j = 0; j < S::DP / 64; ++j) {
           uint2 v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int r = kk * 16 + quad * 2 + (i & 1) + (i >> 1) * 8;
-            v[i] = dg::warp::ld_shared_v2(values + r * S::PITCH + S::swizzled(r, j * 4 + (g >> 1)) * 16 + (g & 1) * 8);
+            const int r = kk * 16 + (i & 1) + (i >> 1) * 8;        // beyond 2 quad
+            const int flip = (S::swizzled(i & 1, j * 4) * 16) & 127;
+            v[i] = dg::warp::ld_shared_v2((at ^ flip) + (j * 64 & ~127) + r * S::PITCH);
           }
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
@@ -753,7 +773,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 
   // Requests without live tokens, dealt over the CTAs.
   for (int b = cta; b < a.batch; b += ctas) {
-    if (live_of<S>(a, b, tid == 0).tiles != 0) continue;
+    if (length_of(a, b, tid == 0) != 0) continue;
     const long long width = static_cast<long long>(a.heads) * a.head_dim;
     for (int h = warp; h < a.heads; h += S::NW)
       for (int d = lane; d < a.head_dim; d += 32) {
@@ -771,11 +791,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
   long long mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const Live v = live_of<S>(a, b, false);
-    if (v.tiles != 0) mine += v.tiles + v.extra;
-  }
-  mine *= items;
+  for (int b = b0; b < b1; ++b) mine += units_of<S>(a, b, items);
   long long scan = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -802,8 +818,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
     long long base = before;
     int b = b0;
     for (;; ++b) {
-      const Live v = live_of<S>(a, b, false);
-      const long long n = v.tiles != 0 ? static_cast<long long>(v.tiles + v.extra) * items : 0;
+      const long long n = units_of<S>(a, b, items);
       if (x0 < base + n) break;
       base += n;
     }
@@ -884,6 +899,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < S::RPT; ++i) {
       const int row = warp + i * S::NW;
+      if (row >= S::ROWS) break;
       float top = kNegInf, l = 0.0f;
 #pragma unroll
       for (int v = 0; v < S::NW; ++v) top = fmaxf(top, warp_m[v * S::ROWS + row]);
@@ -917,6 +933,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 #pragma unroll
       for (int i = 0; i < S::RPT; ++i) {
         const int row = warp + i * S::NW;
+        if (row >= S::ROWS) break;
 #pragma unroll
         for (int c = 0; c < ROUND_CHUNKS; ++c) {
           float v = 0.0f;
@@ -928,11 +945,12 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       }
     }
 
-    const int n_tiles = share.live.tiles;
+    const int n_tiles = share.tiles;
     if (share.count == n_tiles) {              // the whole item
 #pragma unroll
       for (int i = 0; i < S::RPT; ++i)
-        finish_row<S>(p, share.b, share.item, warp + i * S::NW, sum[i], row_m[i], row_l[i], lane);
+        if (warp + i * S::NW < S::ROWS)
+          finish_row<S>(p, share.b, share.item, warp + i * S::NW, sum[i], row_m[i], row_l[i], lane);
       continue;
     }
 
@@ -942,13 +960,14 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < S::RPT; ++i) {
       const int row = warp + i * S::NW;
+      if (row >= S::ROWS) break;
       float* dst = p.share_o + (slot * kMaxRows + row) * kMaxDim + lane;
 #pragma unroll
       for (int c = 0; c < S::CHUNKS; ++c) dst[c * 32] = sum[i][c];
       if (lane == 0) p.share_ml[slot * kMaxRows + row] = make_float2(row_m[i], row_l[i]);
     }
     // The CTAs of the item: those that own its first and its last tile.
-    const long long first_unit = share.item_x0 + share.live.extra;
+    const long long first_unit = x0 + share.x + extra_of<S>(n_tiles);
     const int c0 = static_cast<int>(divided((first_unit + 1) * used - 1, total));
     const int c1 = static_cast<int>(divided((first_unit + n_tiles) * used - 1, total));
     const int n = c1 - c0 + 1;
@@ -968,6 +987,7 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
 #pragma unroll
     for (int i = 0; i < S::RPT; ++i) {
       const int row = warp + i * S::NW;
+      if (row >= S::ROWS) break;
       float top = kNegInf;
       for (int c = lane; c < n; c += 32) {
         const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
