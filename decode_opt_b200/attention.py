@@ -230,8 +230,8 @@ def _heads_of(name: str, t, tokens: int, dim: int, dtype, device):
         raise ValueError(f"{name} must be {dtype} [{tokens}, heads, {dim}] on {device}")
     n, heads, d = t.shape
     s0, s1, unit = t.stride()
-    if n != tokens or d != dim or heads < 1 or unit != 1:
-        raise ValueError(f"{name} must be [{tokens}, heads >= 1, {dim}] with unit last stride")
+    if n != tokens or d != dim or heads < 1 or unit != 1 or max(s0, s1) > 0x1fffffff:
+        raise ValueError(f"{name} must be [{tokens}, heads >= 1, {dim}] with unit last stride and strides below 2^29")
     return heads, (s0, s1)
 
 
@@ -267,9 +267,9 @@ def _rotary(q, k, v, positions, table, sections, interleaved, pairing, inverse, 
     x = q if q is not None else k
     dtype, device = x.dtype, x.device
     kind = _TYPE.get(dtype)
-    _need(kind is not None and x.dim() == 3 and x.shape[0] >= 1,
-          "q and k must be bf16, fp16 or fp32 [tokens >= 1, heads, dim]")
+    _need(kind is not None and x.dim() == 3, "q and k must be bf16, fp16 or fp32 [tokens, heads, dim]")
     tokens, _, dim = x.shape
+    _need(tokens >= 1 and 2 <= dim <= 2048, "q and k need at least one token and a dim of 2 .. 2048")
     heads = kv_heads = code = pages = page_size = 0
     qs = ks = vs = qos = kos = _NO2
     kcs = vcs = _NO3

@@ -5,15 +5,18 @@
 // (include/decode_attention_b200.h gives the definition).
 //
 // Pure traffic: every value is read once and written once, 3 multiply-adds a
-// pair.  The unit of work ("task") is 2 * VE values of one row (a row = one
-// head of one token's q, k or v): the two 16-byte vectors whose values pair
-// up, so that a rotation never crosses threads and an output may be its
-// input.  Tasks are numbered through a token's rows and a CTA takes a group
-// of whole tokens (or, with few tokens, a piece of one), so that neighbouring
-// lanes read neighbouring vectors whatever the head counts are.  cos and sin
-// are fetched once per token and pair into shared memory -- the axes differ
-// from pair to pair, so this is a gather -- and serve all heads from there.
-
+// pair.  A "row" is one head of one token's q, k or v, a "unit" of it 2 * VE
+// values: the two 16-byte vectors whose values pair up, so that a rotation
+// never crosses threads and an output may be its input.  A thread keeps one
+// unit and takes rows in steps, so that neighbouring lanes read neighbouring
+// vectors whatever the head counts are, and has the next row's vectors on the
+// way while it turns one.  cos and sin are fetched once per token and pair
+// into shared memory -- the axes differ from pair to pair, so this is a
+// gather -- and serve all heads from there; a CTA takes several tokens, so that
+// the three loads that follow one another before its first product (position,
+// table, value) are waited for once.  With few tokens a token's rows are dealt
+// over several CTAs, one row a thread.
+//
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -29,7 +32,11 @@
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxTableFloats = 8192;    // cos and sin of one CTA's tokens (32 KiB)
+constexpr int kMaxThreads = 1024;        // a head of 2048 values, one by one
+constexpr int kCtasPerSm = 4;            // 64 registers a thread; 5 (48) spill: 250 -> 336 us for 32768 tokens of 80 heads
+constexpr int kRowsPerThread = 8;        // wanted, with tokens enough
+constexpr int kMaxTokens = 64;           // of a CTA
+constexpr int kMaxTrig = 4096;           // floats of cos and sin of a CTA's tokens (16 KiB)
 
 struct E4m3 {
   uint8_t bits;
@@ -45,6 +52,9 @@ __device__ __forceinline__ void from_float(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_float(E4m3& d, float v) {
   d.bits = static_cast<uint8_t>(__nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3));
 }
+__device__ __forceinline__ uint16_t e4m3_pair(float lo, float hi) {
+  return static_cast<uint16_t>(__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3));
+}
 
 // N values as one access.
 template <typename T, int N>
@@ -58,99 +68,149 @@ __device__ __forceinline__ Vec<T, N> load(const T* p) {
 }
 template <typename T, int N>
 __device__ __forceinline__ void store(T* p, const float (&x)[N]) {
-  Vec<T, N> o;
+  if constexpr (std::is_same<T, E4m3>::value && N % 2 == 0) {
+    Vec<uint16_t, N / 2> o;
 #pragma unroll
-  for (int i = 0; i < N; ++i) from_float(o.v[i], x[i]);
-  *reinterpret_cast<Vec<T, N>*>(p) = o;
+    for (int i = 0; i < N / 2; ++i) o.v[i] = e4m3_pair(x[2 * i], x[2 * i + 1]);
+    *reinterpret_cast<Vec<uint16_t, N / 2>*>(p) = o;
+  } else {
+    Vec<T, N> o;
+#pragma unroll
+    for (int i = 0; i < N; ++i) from_float(o.v[i], x[i]);
+    *reinterpret_cast<Vec<T, N>*>(p) = o;
+  }
 }
 
 struct Geometry {
-  int tokens_per_cta;     // whole tokens a CTA takes
-  int units;              // tasks a row
-  int tasks;              // tasks a token
-  int pieces;             // CTAs a token is split over (tokens_per_cta == 1)
+  int units;              // units a row
   int rows;               // rows a token: heads + kv_heads (k) + kv_heads (v)
+  int slots;              // rows that a CTA's threads cover at once
+  int tokens;             // tokens a CTA takes
+  int pieces;             // CTAs that a token's rows are dealt over (tokens == 1)
+  // Byte strides (token, head): a row's address is two 32 x 32 -> 64 bit
+  // multiply-adds.
+  int q[2], k[2], v[2], q_out[2], k_out[2];
 };
 
+template <typename P>
+__device__ __forceinline__ P* at(P* base, int t, int token_stride, int row, int head_stride) {
+  using Byte = typename std::conditional<std::is_const<P>::value, const char, char>::type;
+  return reinterpret_cast<P*>(reinterpret_cast<Byte*>(base) + static_cast<long long>(t) * token_stride +
+                              static_cast<long long>(row) * head_stride);
+}
+
+// kThreads threads, or for heads of more than 2 * kThreads values that are
+// taken one by one, as many as a row has units.
 template <typename T, typename C, int VE>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ dg_rotary_args a,
-                                                          const Geometry g) {
-  __shared__ __align__(16) float trig[kMaxTableFloats];
+__global__ void __launch_bounds__(VE == 1 ? kMaxThreads : kThreads, VE == 1 ? 1 : kCtasPerSm)
+    rotary_kernel(const __grid_constant__ dg_rotary_args a, const __grid_constant__ Geometry g) {
+  constexpr bool kCached = !std::is_same<C, void>::value;
+  __shared__ __align__(16) float trig[kMaxTrig];     // [token][cos of rot/2 pairs, sin of rot/2 pairs]
+  __shared__ int2 place[kMaxTokens];                 // cache page and offset, page -1: none
+
   dg::sm100::griddep_launch_dependents();
   dg::sm100::griddep_wait();
 
   const int tid = static_cast<int>(threadIdx.x);
+  const int slot = tid / g.units, unit = tid - slot * g.units;
+  const unsigned group = blockIdx.x / static_cast<unsigned>(g.pieces);
+  const int piece = static_cast<int>(blockIdx.x - group * static_cast<unsigned>(g.pieces));
+  const int t0 = static_cast<int>(group) * g.tokens;
+  const int tokens = min(g.tokens, a.tokens - t0);
   const int half = a.rot >> 1;
-  const int group = static_cast<int>(blockIdx.x / static_cast<unsigned>(g.pieces));
-  const int piece = static_cast<int>(blockIdx.x - static_cast<unsigned>(group) * static_cast<unsigned>(g.pieces));
-  const int t0 = group * g.tokens_per_cta;
-  const int tokens = min(g.tokens_per_cta, a.tokens - t0);
+  const int q_rows = a.heads, qk_rows = a.heads + a.kv_heads;
+  const bool rotates = unit < a.rot / (2 * VE);
+  // A unit's two vectors in a row that turns, and in one that passes (v).
+  const int first_r = rotates && a.pairing == DG_PAIR_HALF ? unit * VE : unit * 2 * VE;
+  const int second_r = rotates && a.pairing == DG_PAIR_HALF ? first_r + half : first_r + VE;
+  const int first_v = unit * 2 * VE, second_v = first_v + VE;
 
-  // trig[token][0, half) = cos, [half, rot) = +-sin of that pair's axis.
-  for (int i = tid; i < tokens * half; i += kThreads) {
-    const int tok = i / half, pair = i - tok * half;
+  auto fetch = [&](int tok, int row, Vec<T, VE>& lo, Vec<T, VE>& hi) {
+    const bool is_q = row < q_rows, is_v = row >= qk_rows;
+    const T* src = at(static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k), t0 + tok,
+                      is_q ? g.q[0] : is_v ? g.v[0] : g.k[0], row - (is_q ? 0 : is_v ? qk_rows : q_rows),
+                      is_q ? g.q[1] : is_v ? g.v[1] : g.k[1]);
+    const int second = is_v ? second_v : second_r;
+    lo = load<T, VE>(src + (is_v ? first_v : first_r));
+    if (second < a.head_dim) hi = load<T, VE>(src + second);
+  };
+  // (tok, row) -> this thread's next.
+  const int step = g.slots * g.pieces;
+  auto next = [&](int& tok, int& row) {
+    row += step;
+    while (row >= g.rows && tok < tokens) {
+      row -= g.rows;
+      ++tok;
+    }
+  };
+
+  int tok = 0, row = slot + piece * g.slots - step;
+  next(tok, row);
+  if (g.pieces > 1 && tok > 0) tok = tokens;         // a dealt token's rows are done in one round
+  const bool idle = slot >= g.slots;
+  Vec<T, VE> lo{}, hi{};
+  if (!idle && tok < tokens) fetch(tok, row, lo, hi);
+
+  for (int i = tid; i < tokens * half; i += static_cast<int>(blockDim.x)) {
+    const int tk = i / half, pair = i - tk * half;
     const int axis = (a.axis_of[pair >> 4] >> ((pair & 15) * 2)) & 3;
-    const long long at = axis * a.position_stride + t0 + tok;
-    const long long p = a.position_64 != 0 ? static_cast<const long long*>(a.positions)[at]
-                                           : static_cast<const int*>(a.positions)[at];
+    const long long from = axis * a.position_stride + t0 + tk;
+    const long long p = a.position_64 != 0 ? static_cast<const long long*>(a.positions)[from]
+                                           : static_cast<const int*>(a.positions)[from];
     float c = __int_as_float(0x7fffffff), s = c;     // NaN
     if (p >= 0 && p < a.max_position) {
-      const float* row = a.cos_sin + p * a.rot;
-      c = __ldg(row + pair);
-      s = __ldg(row + half + pair);
+      c = __ldg(a.cos_sin + p * a.rot + pair);
+      s = __ldg(a.cos_sin + p * a.rot + half + pair);
     } else if (a.status != nullptr) {
       atomicCAS(a.status, 0, DG_ERR_POSITION);
     }
-    trig[tok * a.rot + pair] = c;
-    trig[tok * a.rot + half + pair] = a.inverse != 0 ? -s : s;
+    trig[tk * a.rot + pair] = c;
+    trig[tk * a.rot + half + pair] = a.inverse != 0 ? -s : s;
+  }
+  if constexpr (kCached) {
+    for (int i = tid; i < tokens; i += static_cast<int>(blockDim.x)) {
+      const long long row_at = a.slots[t0 + i];
+      long long page = -1, offset = 0;
+      if (row_at >= static_cast<long long>(a.num_pages) * a.page_size) {
+        if (a.status != nullptr) atomicCAS(a.status, 0, DG_ERR_SLOT);
+      } else if (row_at >= 0) {
+        page = (row_at >> 32) == 0 ? static_cast<unsigned>(row_at) / static_cast<unsigned>(a.page_size)
+                                   : row_at / a.page_size;
+        offset = row_at - page * a.page_size;
+      }
+      place[i] = make_int2(static_cast<int>(page), static_cast<int>(offset));
+    }
   }
   __syncthreads();
+  if (idle) return;
 
-  const int rotated_units = a.rot / (2 * VE);
-  const int all = tokens * g.tasks;
-  for (int i = tid + piece * kThreads; i < all; i += kThreads * g.pieces) {
-    const int tok = i / g.tasks, task = i - tok * g.tasks;
-    const int row = task / g.units, unit = task - row * g.units;
-    const long long t = t0 + tok;
-    const bool is_q = row < a.heads;
-    const bool is_v = row >= a.heads + a.kv_heads;
-    const int head = is_q ? row : (is_v ? row - a.heads - a.kv_heads : row - a.heads);
-
-    const T* src = is_q ? static_cast<const T*>(a.q) + t * a.q_stride[0] + head * a.q_stride[1]
-                        : is_v ? static_cast<const T*>(a.v) + t * a.v_stride[0] + head * a.v_stride[1]
-                               : static_cast<const T*>(a.k) + t * a.k_stride[0] + head * a.k_stride[1];
-    // The task's two vectors.
-    const bool turns = !is_v && unit < rotated_units;
-    const int first = turns ? (a.pairing == DG_PAIR_HALF ? unit * VE : unit * 2 * VE) : unit * 2 * VE;
-    const int second = turns && a.pairing == DG_PAIR_HALF ? first + half : first + VE;
-    const bool both = second < a.head_dim;   // a row's last passing vector can stand alone
+  while (tok < tokens) {
+    const int r = row, tk = tok;
+    const bool is_q = r < q_rows, is_v = r >= qk_rows;
+    const int first = is_v ? first_v : first_r, second = is_v ? second_v : second_r;
+    const bool both = second < a.head_dim;           // a row's last passing vector can stand alone
     float x[VE], y[VE];
-    {
-      const Vec<T, VE> lo = load<T, VE>(src + first);
 #pragma unroll
-      for (int j = 0; j < VE; ++j) x[j] = to_float(lo.v[j]);
-      if (both) {
-        const Vec<T, VE> hi = load<T, VE>(src + second);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) y[j] = to_float(hi.v[j]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < VE; ++j) y[j] = 0.0f;
-      }
+    for (int j = 0; j < VE; ++j) {
+      x[j] = to_float(lo.v[j]);
+      y[j] = both ? to_float(hi.v[j]) : 0.0f;
     }
-    if (turns) {
-      const Vec<float, (VE < 4 ? VE : 4)>* cs;
+    next(tok, row);
+    if (g.pieces > 1) tok = tokens;
+    if (tok < tokens) fetch(tok, row, lo, hi);
+
+    if (rotates && !is_v) {
       float c[VE], s[VE];
-      const float* base = trig + tok * a.rot + unit * VE;
+      const float* cs = trig + tk * a.rot + unit * VE;
       constexpr int W = VE < 4 ? VE : 4;
 #pragma unroll
       for (int j = 0; j < VE; j += W) {
-        cs = reinterpret_cast<const Vec<float, W>*>(base + j);
+        const Vec<float, W> u = load<float, W>(cs + j), w = load<float, W>(cs + half + j);
 #pragma unroll
-        for (int l = 0; l < W; ++l) c[j + l] = cs->v[l];
-        cs = reinterpret_cast<const Vec<float, W>*>(base + half + j);
-#pragma unroll
-        for (int l = 0; l < W; ++l) s[j + l] = cs->v[l];
+        for (int l = 0; l < W; ++l) {
+          c[j + l] = u.v[l];
+          s[j + l] = w.v[l];
+        }
       }
       if (a.pairing == DG_PAIR_HALF) {
 #pragma unroll
@@ -180,30 +240,23 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
         }
       }
     }
-    T* dst = is_q ? (a.q_out != nullptr ? static_cast<T*>(a.q_out) + t * a.q_out_stride[0] + head * a.q_out_stride[1]
-                                        : nullptr)
-                  : (!is_v && a.k_out != nullptr
-                         ? static_cast<T*>(a.k_out) + t * a.k_out_stride[0] + head * a.k_out_stride[1]
-                         : nullptr);
-    if (dst != nullptr) {
+    if (is_q || (!is_v && a.k_out != nullptr)) {
+      T* dst = at(static_cast<T*>(is_q ? a.q_out : a.k_out), t0 + tk, is_q ? g.q_out[0] : g.k_out[0],
+                  is_q ? r : r - q_rows, is_q ? g.q_out[1] : g.k_out[1]);
       store<T, VE>(dst + first, x);
       if (both) store<T, VE>(dst + second, y);
     }
-    if constexpr (!std::is_same<C, void>::value) {
-      if (is_q) continue;
-      const long long slot = a.slots[t];
-      if (slot < 0) continue;
-      if (slot >= static_cast<long long>(a.num_pages) * a.page_size) {
-        if (a.status != nullptr) atomicCAS(a.status, 0, DG_ERR_SLOT);
-        continue;
-      }
-      const long long page = slot / a.page_size, offset = slot - page * a.page_size;
+    if constexpr (kCached) {
+      const int2 where = place[tk];
+      if (is_q || where.x < 0) continue;
+      const int head = r - (is_v ? qk_rows : q_rows);
       const long long* st = is_v ? a.v_cache_stride : a.k_cache_stride;
-      C* cache = static_cast<C*>(is_v ? a.v_cache : a.k_cache) + page * st[0] + offset * st[1] + head * st[2];
+      C* cache = static_cast<C*>(is_v ? a.v_cache : a.k_cache) + where.x * st[0] + where.y * st[1] +
+                 head * st[2];
       if constexpr (std::is_same<C, E4m3>::value) {
         const float* scales = is_v ? a.v_scale : a.k_scale;
         if (scales != nullptr) {
-          const float scale = scales[head];
+          const float scale = __ldg(scales + head);
 #pragma unroll
           for (int j = 0; j < VE; ++j) {
             x[j] = x[j] / scale;
@@ -218,6 +271,16 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
 }
 
 bool multiple(long long stride, int n) { return stride % n == 0; }
+
+// Byte strides of one tensor as ints; false where they do not fit.
+bool bytes_of(const void* p, const long long (&stride)[2], int size, int (&out)[2]) {
+  for (int i = 0; i < 2; ++i) {
+    const long long b = p == nullptr ? 0 : stride[i] * size;
+    if (b < 0 || b > 0x7fffffffLL) return false;
+    out[i] = static_cast<int>(b);
+  }
+  return true;
+}
 
 // Whether every access can be `ve` values wide.
 bool fits(const dg_rotary_args& a, int ve, int size, int cache_size) {
@@ -270,7 +333,7 @@ Kernel pick(const dg_rotary_args& a, int cache_size, int* ve) {
 }
 
 bool refused(const dg_rotary_args& a) {
-  if (a.tokens < 1 || a.heads < 0 || a.kv_heads < 0 || a.heads + a.kv_heads < 1 || a.head_dim < 2 || a.rot < 2 ||
+  if (a.tokens < 1 || a.heads < 0 || a.kv_heads < 0 || a.heads + a.kv_heads < 1 || a.head_dim < 2 || a.head_dim > 2 * kMaxThreads || a.rot < 2 ||
       a.rot % 2 != 0 || a.rot > a.head_dim || a.rot > DG_MAX_ROT || a.max_position < 1)
     return true;
   if (a.type != DG_TYPE_BF16 && a.type != DG_TYPE_FP16 && a.type != DG_TYPE_FP32) return true;
@@ -303,29 +366,43 @@ extern "C" int dg_rotary(const dg_rotary_args* args, void* stream, int pdl_attr)
   if (fn == nullptr) return cudaErrorInvalidValue;
 
   Geometry g;
+  const int size = a.type == DG_TYPE_FP32 ? 4 : 2;
+  if (!bytes_of(a.q, a.q_stride, size, g.q) || !bytes_of(a.k, a.k_stride, size, g.k) ||
+      !bytes_of(a.v, a.v_stride, size, g.v) || !bytes_of(a.q_out, a.q_out_stride, size, g.q_out) ||
+      !bytes_of(a.k_out, a.k_out_stride, size, g.k_out))
+    return cudaErrorInvalidValue;
   const long long rows = static_cast<long long>(a.heads) + a.kv_heads + (a.v != nullptr ? a.kv_heads : 0);
+  if (rows > (1 << 24)) return cudaErrorInvalidValue;
   g.units = (a.head_dim + 2 * ve - 1) / (2 * ve);
-  const long long tasks = rows * g.units;
-  if (tasks > (1 << 24)) return cudaErrorInvalidValue;
+  const int threads = g.units <= kThreads ? kThreads : (g.units + 31) / 32 * 32;
   g.rows = static_cast<int>(rows);
-  g.tasks = static_cast<int>(tasks);
-  // About two tasks a thread: whole tokens while there are CTAs enough, else
-  // a token's tasks spread over several CTAs so that a decode step uses more
-  // than `tokens` SMs.
+  g.slots = threads / g.units;
+  // A decode step has fewer tokens than the GPU has SMs: one row a thread
+  // then, so that its latency is one row's.  Else whole tokens, about
+  // kRowsPerThread rows a thread, in whole waves of the GPU.
   const int sms = dg_num_sms() > 0 ? dg_num_sms() : 148;
-  g.tokens_per_cta = static_cast<int>(2 * kThreads / tasks);
-  if (g.tokens_per_cta > kMaxTableFloats / a.rot) g.tokens_per_cta = kMaxTableFloats / a.rot;
-  if (g.tokens_per_cta < 1 || a.tokens <= 2 * sms) g.tokens_per_cta = 1;
   g.pieces = 1;
-  if (a.tokens <= 2 * sms) g.pieces = static_cast<int>((tasks + kThreads - 1) / kThreads);
-  const long long groups = (static_cast<long long>(a.tokens) + g.tokens_per_cta - 1) / g.tokens_per_cta;
+  g.tokens = 1;
+  if (a.tokens <= 2 * sms) {
+    g.pieces = (g.rows + g.slots - 1) / g.slots;
+  } else {
+    const long long wanted = (static_cast<long long>(g.slots) * kRowsPerThread + g.rows - 1) / g.rows;
+    const long long places = static_cast<long long>(sms) * kCtasPerSm;
+    long long waves = a.tokens / (places * wanted);
+    if (waves < 1) waves = 1;
+    const long long tokens = (a.tokens + places * waves - 1) / (places * waves);
+    g.tokens = static_cast<int>(tokens < kMaxTokens ? tokens : kMaxTokens);
+    if (g.tokens > kMaxTrig / a.rot) g.tokens = kMaxTrig / a.rot;
+    if (g.tokens < 1) g.tokens = 1;
+  }
+  const long long groups = (static_cast<long long>(a.tokens) + g.tokens - 1) / g.tokens;
   const long long ctas = groups * g.pieces;
   if (ctas > 0x7fffffffLL) return cudaErrorInvalidValue;
 
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1]{};
   cfg.gridDim = dim3(static_cast<unsigned>(ctas), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cfg.attrs = attr;
   cfg.numAttrs = 0;

@@ -101,7 +101,7 @@ int dg_build_block_tables(const dg_block_tables* args, void* stream, int pdl_att
 typedef struct dg_rotary_args {
   int tokens;                /* T >= 1                                                           */
   int heads, kv_heads;       /* of q (0 without q) and of k and v (0 without k)                  */
-  int head_dim;              /* >= 2                                                             */
+  int head_dim;              /* 2 .. 2048                                                        */
   int rot;                   /* even, 2 .. min(head_dim, DG_MAX_ROT)                             */
   int type;                  /* of q, k, v and the outputs: bf16, fp16, fp32                     */
   int cache_type;            /* of the caches: `type` (not fp32) or e4m3                         */
@@ -113,8 +113,8 @@ typedef struct dg_rotary_args {
   const void *q, *k, *v;
   void *q_out, *k_out;
   void *k_cache, *v_cache;   /* [num_pages, page_size, kv_heads, head_dim]                       */
-  long long q_stride[2], k_stride[2], v_stride[2];      /* token, head                           */
-  long long q_out_stride[2], k_out_stride[2];
+  long long q_stride[2], k_stride[2], v_stride[2];      /* token, head: 0 .. 2^31 - 1 bytes each */
+  long long q_out_stride[2], k_out_stride[2];           /* the same                              */
   long long k_cache_stride[3], v_cache_stride[3];       /* page, offset in the page, head        */
   const void* positions;     /* [axes, T]                                                        */
   long long position_stride; /* between axes (0: every axis reads the same)                      */

@@ -86,12 +86,12 @@ def _rotary(**kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(tokens=0), dict(head_dim=1), dict(rot=0), dict(rot=3), dict(rot=66), dict(head_dim=1024, rot=514),
+    dict(tokens=0), dict(head_dim=1), dict(head_dim=2050), dict(rot=0), dict(rot=3), dict(rot=66), dict(head_dim=1024, rot=514),
     dict(max_position=0), dict(type=_lib.TYPE_E4M3), dict(type=_lib.TYPE_FP32), dict(type=7), dict(pairing=2),
     dict(positions=None), dict(cos_sin=None), dict(position_stride=-1), dict(q=None), dict(q_out=None), dict(heads=0),
     dict(k=None), dict(v=None), dict(k_cache=None), dict(v_cache=None), dict(slots=None), dict(page_size=0),
     dict(num_pages=0), dict(cache_type=_lib.TYPE_FP16), dict(k_scale=16), dict(v_scale=16), dict(heads=-1),
-    dict(k_cache=None, v_cache=None, v=None)])
+    dict(k_cache=None, v_cache=None, v=None), dict(q_stride=(1 << 30, 64)), dict(v_stride=(-128, 64))])
 def test_rotary_refusals(kw):
     assert _rotary(**kw) == BAD
 
