@@ -72,9 +72,9 @@ typedef struct dg_block_tables {
   int* block_table;          /* [batch, table_width]                                             */
   int* seq_lens;             /* [batch]; not context_lens or new_lens                            */
   int* query_start;          /* [batch + 1]                                                      */
-  long long* slots;          /* [num_tokens], 16-byte aligned                                    */
-  int* positions;            /* [num_tokens], 16-byte aligned                                    */
-  int* requests;             /* [num_tokens], 16-byte aligned                                    */
+  long long* slots;          /* [num_tokens]                                                     */
+  int* positions;            /* [num_tokens]                                                     */
+  int* requests;             /* [num_tokens]                                                     */
   int* cursor_out;           /* [1]; not cursor_in                                               */
   int* status;
 } dg_block_tables;

@@ -68,7 +68,7 @@ def _tables(**kw):
     dict(batch=0), dict(batch=16385), dict(page_size=0), dict(table_width=0), dict(num_tokens=-1), dict(free_count=-1),
     dict(table_stride=3), dict(context_lens=None), dict(new_lens=None), dict(free_pages=None), dict(block_table=None),
     dict(seq_lens=None), dict(query_start=None), dict(cursor_out=None), dict(slots=None), dict(positions=None),
-    dict(requests=None), dict(slots=120), dict(positions=132), dict(requests=148), dict(seq_lens=16), dict(seq_lens=32),
+    dict(requests=None), dict(slots=116), dict(seq_lens=16), dict(seq_lens=32),
     dict(cursor_in=160)])
 def test_block_tables_refusals(kw):
     assert _tables(**kw) == BAD
