@@ -296,9 +296,9 @@ def lib():
     L.dg_ipc_release.argtypes = [ctypes.c_void_p]
     L.dg_probe_mma.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int,
                                ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]
-    # A struct by reference, or its bytes.
-    for name in ("dg_build_block_tables", "dg_rotary", "dg_paged_attention"):
-        getattr(L, name).argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int]
+    L.dg_build_block_tables.argtypes = [ctypes.POINTER(DgBlockTables), ctypes.c_void_p, ctypes.c_int]
+    L.dg_rotary.argtypes = [ctypes.POINTER(DgRotaryArgs), ctypes.c_void_p, ctypes.c_int]
+    L.dg_paged_attention.argtypes = [ctypes.POINTER(DgAttentionArgs), ctypes.c_void_p, ctypes.c_int]
     L.dg_attention_workspace_bytes.restype = ctypes.c_ulonglong
     if L.dg_abi_version() != ABI_VERSION:
         raise RuntimeError(f"{LIB_PATH}: ABI version {L.dg_abi_version()} != {ABI_VERSION}")

@@ -8,6 +8,11 @@ the CUDA runtime statically and resolves ``cuTensorMapEncodeTiled``
 through the runtime's driver entry-point query, so it loads on hosts without a
 GPU (the CPU test suite checks its exported symbols there).
 
+``csrc/dg_torch.cpp`` becomes ``decode_opt_b200/_host.so``, the extension
+module through which ``attention.py`` makes the attention operators' calls
+(host code against torch's C++ headers; it is handed the library's entry
+points and links no CUDA code of its own).
+
 It then compiles ``tests/cpp/dg_drop_in_check.cu`` against the C++ headers
 (``include/decode_gemm.cuh``, ``include/weight_prepack.cuh``) and the
 library into ``decode_opt_b200/dg_drop_in_check``, the program the GPU tests
@@ -30,6 +35,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB_NAME = "libdecode_gemm_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
+HOST_SRC = os.path.join(CSRC, "dg_torch.cpp")
+HOST_LIB = os.path.join(HERE, "_host.so")
 DROP_IN_SRC = os.path.join(ROOT, "tests", "cpp", "dg_drop_in_check.cu")
 DROP_IN_BIN = os.path.join(HERE, "dg_drop_in_check")
 CUBLASLT_SRC = os.path.join(CSRC, "dg_cublaslt_fp8.cu")
@@ -62,6 +69,29 @@ def build(verbose: bool = False, ptxas_verbose: bool = False, force: bool = Fals
     build_drop_in_check(verbose, force)
     build_cublaslt_bench(verbose, force)
     return lib
+
+
+def build_host(verbose: bool = False, force: bool = False) -> str:
+    """The extension module of the attention operators' calls."""
+    header = os.path.join(INCLUDE, "decode_attention_b200.h")
+    if not force and os.path.exists(HOST_LIB) and \
+            os.path.getmtime(HOST_LIB) > max(os.path.getmtime(HOST_SRC), os.path.getmtime(header)):
+        return HOST_LIB
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    flags = [f"-I{os.path.join(root, 'include')}", f"-I{os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include')}",
+             f"-I{sysconfig.get_paths()['include']}", f"-I{os.path.join(cuda_lib_dir(), '..', 'include')}", f"-I{INCLUDE}"]
+    cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *flags, HOST_SRC, "-o",
+           HOST_LIB + ".tmp", "-L", os.path.join(root, "lib"), "-L", cuda_lib_dir(), "-lc10", "-lc10_cuda", "-ltorch",
+           "-ltorch_cpu", "-ltorch_python", "-lcudart"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(HOST_LIB + ".tmp", HOST_LIB)
+    return HOST_LIB
 
 
 def cuda_lib_dir() -> str:
@@ -97,6 +127,8 @@ def build_drop_in_check(verbose: bool = False, force: bool = False) -> str:
 
 
 def build_library(verbose: bool = False, ptxas_verbose: bool = False, force: bool = False) -> str:
+    """The library and the extension module that calls it from torch."""
+    build_host(verbose, force)
     if not force and not needs_build():
         return LIB_PATH
     cmd = [nvcc(), "-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS,
