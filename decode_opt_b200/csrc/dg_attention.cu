@@ -120,6 +120,9 @@ struct Shape {
   // 2^kBias is the probability of the maximum: fp16's subnormals start at
   // 2^-14, so its probabilities are lifted out of them.
   static constexpr float kBias = sizeof(MM_) != 0 && __is_same(MM_, Fp16) ? 10.0f : 0.0f;
+  // How far a score may pass the reference exponent: 2^(kLag + kBias) stays
+  // well inside fp16.
+  static constexpr float kLag = 5.0f;
   static constexpr size_t SMEM = RING + sizeof(float) * (JOIN + 2 * NW * ROWS_) +
                                  sizeof(uint32_t) * NW * STAGES;
   static_assert(NW * ROWS_ * JOIN_COLS <= JOIN && SMEM <= 227 * 1024 - 1024, "shared memory");
@@ -530,21 +533,27 @@ struct Warp {
         for (int i = 0; i < 2 * R; ++i)
           if (((live >> (t * 8 + quad * 2 + (i & 1))) & 1u) == 0u) s[t][i] = kNegInf;
     }
+    // The reference exponent m follows the maximum only when it falls kLag
+    // behind (probabilities up to 2^(kLag + kBias) are as exact as others), so
+    // that the sums so far are seldom scaled; the first tile has none.
     float alpha[R];
     bool moved = false;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      float top = m[r];
+      float top = s[0][2 * r];
 #pragma unroll
       for (int t = 0; t < S::NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) top = fmaxf(top, s[t][2 * r + i]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      moved = moved || top > m[r];
-      const float from = (top == kNegInf ? 0.0f : top) - S::kBias;
-      alpha[r] = dg::warp::exp2_approx((m[r] - top) == (m[r] - top) ? m[r] - top : kNegInf);
-      m[r] = top;
+      alpha[r] = 1.0f;
+      if (top > m[r] + S::kLag || m[r] == kNegInf) {
+        moved = moved || m[r] != kNegInf;
+        alpha[r] = m[r] == kNegInf ? 0.0f : dg::warp::exp2_approx(m[r] - top);
+        m[r] = top;
+      }
+      const float from = (m[r] == kNegInf ? 0.0f : m[r]) - S::kBias;
       float sum = 0.0f;
 #pragma unroll
       for (int t = 0; t < S::NT; ++t)
@@ -578,7 +587,9 @@ struct Warp {
           const uint32_t top = S::MM::cut(u, v);
           const float2 back = S::MM::unpack(top);
           hi[h * R + r] = top;
-          lo[h * R + r] = S::MM::pack(fmaxf(u - back.x, S::MM::kTiny), fmaxf(v - back.y, S::MM::kTiny));
+          // (e4m3 has no infinity to keep)
+          lo[h * R + r] = S::kE4m3 ? S::MM::pack(u - back.x, v - back.y)
+                                   : S::MM::pack(fmaxf(u - back.x, S::MM::kTiny), fmaxf(v - back.y, S::MM::kTiny));
         }
       uint32_t x[4], y[4];
       if constexpr (R == 1) {
