@@ -116,6 +116,7 @@ struct Shape {
   static constexpr int KS = DP_ / 16;                            // inner steps of Q K^T
   static constexpr int OT = DP_ / 8;                             // output tiles of 8 columns
   static constexpr int CHUNKS = DP_ / 32;                        // of the joins
+  static constexpr int PACK = CHUNKS < 4 ? CHUNKS : 4;           // floats of a share's access
   static constexpr int RPT = (ROWS_ + NW - 1) / NW;              // rows a warp finishes: warp, warp + NW, ...
   // 2^kBias is the probability of the maximum: fp16's subnormals start at
   // 2^-14, so its probabilities are lifted out of them.
@@ -660,6 +661,30 @@ __device__ __forceinline__ void store_out(const dg_attention_args& a, long long 
     static_cast<__half*>(a.out)[at] = __float2half_rn(v);
 }
 
+// N floats of a share as one access; loads past L1, where another CTA's share
+// of the launch before may lie.
+template <int N>
+__device__ __forceinline__ void store_pack(float* to, const float* x) {
+  if constexpr (N == 4)
+    *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+  else
+    *reinterpret_cast<float2*>(to) = make_float2(x[0], x[1]);
+}
+template <int N>
+__device__ __forceinline__ void load_pack(const float* from, float (&x)[N]) {
+  if constexpr (N == 4) {
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(from));
+    x[0] = v.x;
+    x[1] = v.y;
+    x[2] = v.z;
+    x[3] = v.w;
+  } else {
+    const float2 v = __ldcg(reinterpret_cast<const float2*>(from));
+    x[0] = v.x;
+    x[1] = v.y;
+  }
+}
+
 // A finished row: this lane's column of each 32-column chunk, unnormalised.
 template <typename S>
 __device__ __forceinline__ void finish_row(const Params& p, int b, int item, int row, const float (&v)[S::CHUNKS],
@@ -762,6 +787,25 @@ __device__ __forceinline__ void finish_solo(const Params& p, int b, int item, co
   }
 }
 
+// Requests without live tokens, dealt over the CTAs.
+template <typename S>
+__device__ __forceinline__ void finish_empty(const dg_attention_args& a, int cta, int ctas, int tid) {
+  const int lane = tid & 31, warp = tid >> 5;
+  const long long width = static_cast<long long>(a.heads) * a.head_dim;
+  for (int b = cta; b < a.batch; b += ctas) {
+    if (length_of(a, b, tid == 0) != 0) continue;
+    for (int h = warp; h < a.heads; h += S::NW)
+      for (int d = lane; d < a.head_dim; d += 32) {
+        store_out(a, b * a.out_stride[0] + h * a.out_stride[1] + d, 0.0f);
+        if (a.q_out != nullptr) static_cast<uint8_t*>(a.q_out)[b * width + h * a.head_dim + d] = 0;
+      }
+    for (int h = tid; h < a.heads && a.lse != nullptr; h += S::NW * 32)
+      a.lse[static_cast<long long>(b) * a.heads + h] = kNegInf;
+    for (int i = tid; i < width / 128 && a.q_out != nullptr; i += S::NW * 32)
+      a.q_scales[b * (width / 128) + i] = kQuantEps / kFp8Max;
+  }
+}
+
 template <typename S>
 __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -781,21 +825,6 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   constexpr int kThreads = S::NW * 32;
   const int cta = static_cast<int>(blockIdx.x), ctas = static_cast<int>(gridDim.x);
   const int items = a.kv_heads * p.groups;
-
-  // Requests without live tokens, dealt over the CTAs.
-  for (int b = cta; b < a.batch; b += ctas) {
-    if (length_of(a, b, tid == 0) != 0) continue;
-    const long long width = static_cast<long long>(a.heads) * a.head_dim;
-    for (int h = warp; h < a.heads; h += S::NW)
-      for (int d = lane; d < a.head_dim; d += 32) {
-        store_out(a, b * a.out_stride[0] + h * a.out_stride[1] + d, 0.0f);
-        if (a.q_out != nullptr) static_cast<uint8_t*>(a.q_out)[b * width + h * a.head_dim + d] = 0;
-      }
-    for (int h = tid; h < a.heads && a.lse != nullptr; h += kThreads)
-      a.lse[static_cast<long long>(b) * a.heads + h] = kNegInf;
-    for (int i = tid; i < width / 128 && a.q_out != nullptr; i += kThreads)
-      a.q_scales[b * (width / 128) + i] = kQuantEps / kFp8Max;
-  }
 
   // The line of tiles: its length, and the request where this CTA's run
   // begins.
@@ -822,7 +851,10 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   }
   // CTAs in use, and this one's run [x0, x1) of the line.
   const int used = static_cast<int>(min(static_cast<long long>(ctas), (total + S::MIN_RUN - 1) / S::MIN_RUN));
-  if (cta >= used) return;
+  if (cta >= used) {
+    finish_empty<S>(a, cta, ctas, tid);
+    return;
+  }
   const long long x0 = static_cast<long long>(divided(total * cta, used));
   const long long x1 = static_cast<long long>(divided(total * (cta + 1), used));
   if (before <= x0 && x0 < before + mine) {
@@ -972,9 +1004,10 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
     for (int i = 0; i < S::RPT; ++i) {
       const int row = warp + i * S::NW;
       if (row >= S::ROWS) break;
-      float* dst = p.share_o + (slot * kMaxRows + row) * kMaxDim + lane;
+      // A lane's columns side by side.
+      float* dst = p.share_o + (slot * kMaxRows + row) * kMaxDim + lane * S::CHUNKS;
 #pragma unroll
-      for (int c = 0; c < S::CHUNKS; ++c) dst[c * 32] = sum[i][c];
+      for (int c = 0; c < S::CHUNKS; c += S::PACK) store_pack<S::PACK>(dst + c, &sum[i][c]);
       if (lane == 0) p.share_ml[slot * kMaxRows + row] = make_float2(row_m[i], row_l[i]);
     }
     // The CTAs of the item: those that own its first and its last tile.
@@ -983,12 +1016,10 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
     const int c1 = static_cast<int>(divided((first_unit + n_tiles) * used - 1, total));
     const int n = c1 - c0 + 1;
     __syncthreads();
-    if (tid == 0) {
-      __threadfence();
+    if (tid == 0) {                         // releases the CTA's share, acquires the others'
       const int seen = dg::sm100::atomic_add_acq_rel_gpu(p.tickets + c0, 1);
       is_last = seen == n - 1;
       if (seen == n - 1) dg::sm100::store_relaxed_gpu(p.tickets + c0, 0);   // ready for the next launch
-      __threadfence();
     }
     __syncthreads();
     if (is_last == 0) continue;
@@ -999,20 +1030,25 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
     for (int i = 0; i < S::RPT; ++i) {
       const int row = warp + i * S::NW;
       if (row >= S::ROWS) break;
+      constexpr int PER_LANE = (kMaxCtas + 31) / 32;
+      float2 ml[PER_LANE];
       float top = kNegInf;
-      for (int c = lane; c < n; c += 32) {
+#pragma unroll
+      for (int k = 0; k < PER_LANE; ++k) {
+        const int c = lane + k * 32;
         const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
-        top = fmaxf(top, __ldcg(p.share_ml + from * kMaxRows + row).x);
+        ml[k] = c < n ? __ldcg(p.share_ml + from * kMaxRows + row) : make_float2(kNegInf, 0.0f);
       }
+#pragma unroll
+      for (int k = 0; k < PER_LANE; ++k) top = fmaxf(top, ml[k].x);
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
       float l = 0.0f;
-      for (int c = lane; c < n; c += 32) {
-        const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
-        const float2 ml = __ldcg(p.share_ml + from * kMaxRows + row);
-        const float f = ml.x == kNegInf ? 0.0f : dg::warp::exp2_approx(ml.x - top);
-        by[row * kMaxCtas + c] = f;
-        l += f * ml.y;
+#pragma unroll
+      for (int k = 0; k < PER_LANE; ++k) {
+        const float f = ml[k].x == kNegInf ? 0.0f : dg::warp::exp2_approx(ml[k].x - top);
+        if (lane + k * 32 < n) by[row * kMaxCtas + lane + k * 32] = f;
+        l += f * ml[k].y;
       }
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
@@ -1020,19 +1056,25 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       float v[S::CHUNKS];
 #pragma unroll
       for (int c = 0; c < S::CHUNKS; ++c) v[c] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
       for (int c = 0; c < n; ++c) {
         const size_t from = 2 * static_cast<size_t>(c0 + c) + (c == 0 ? 1 : 0);
-        const float* src = p.share_o + (from * kMaxRows + row) * kMaxDim + lane;
+        const float* src = p.share_o + (from * kMaxRows + row) * kMaxDim + lane * S::CHUNKS;
         const float f = by[row * kMaxCtas + c];
 #pragma unroll
-        for (int k = 0; k < S::CHUNKS; ++k) v[k] += f * __ldcg(src + k * 32);
+        for (int k = 0; k < S::CHUNKS; k += S::PACK) {
+          float x[S::PACK];
+          load_pack<S::PACK>(src + k, x);
+#pragma unroll
+          for (int j = 0; j < S::PACK; ++j) v[k + j] += f * x[j];
+        }
       }
       finish_row<S>(p, share.b, share.item, row, v, top, l, lane);
     }
     __syncthreads();                        // the join buffers and is_last are free again
   }
   dg::warp::cp_async_wait<0>();
+  finish_empty<S>(a, cta, ctas, tid);
 }
 
 using Kernel = void (*)(const Params);
