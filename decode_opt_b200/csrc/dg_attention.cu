@@ -110,7 +110,11 @@ struct Shape {
   static constexpr int JOIN_COLS =                               // columns a round: a power of two from 32
       NW * ROWS_ * DP_ <= JOIN ? DP_ : NW * ROWS_ * 128 <= JOIN ? 128 : NW * ROWS_ * 64 <= JOIN ? 64 : 32;
   static constexpr int SOLO = 8;                                 // tiles of an item that one warp does alone
-  static constexpr int EXTRA_SOLO = 1, EXTRA = 8;                // an item's cost in tiles, beyond its tiles
+  // What an item costs beyond its tiles (join, uneven warps), in tiles: CTAs
+  // with 3 and with 15 items of the same units differed by 1.7 to 4.5 us an
+  // item.  Ragged batch, 8 heads an item: 129.8 us at 4, 123.7 at 8, 123.0 at
+  // 14, 122.7 at 20; 16 heads: 161.7, 149.9, 142.1, 135.4.
+  static constexpr int EXTRA_SOLO = 1, EXTRA = ROWS_ == 8 ? 14 : 20;
   static constexpr int MIN_RUN = 4;                              // units a CTA takes at least
   static constexpr int NT = TOK / 8;                             // score tiles of 8 tokens
   static constexpr int KS = DP_ / 16;                            // inner steps of Q K^T

@@ -130,7 +130,7 @@ def test_null_arguments_are_refused():
     assert L.dg_paged_attention(None, None, 0) == BAD
 
 
-def _cut(lens, items, tok, window, ctas, warps, extra=8, extra_solo=1, min_run=4):
+def _cut(lens, items, tok, window, ctas, warps, extra=14, extra_solo=1, min_run=8):
     """The attention kernel's cut of a batch: (units, CTAs in use, per CTA its
     shares (request, item, first tile, tiles, unit of the item's first tile,
     the item's tiles, one warp's work or not))."""
