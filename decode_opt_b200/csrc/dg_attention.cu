@@ -115,7 +115,7 @@ struct Shape {
   // item.  Ragged batch, 8 heads an item: 129.8 us at 4, 123.7 at 8, 123.0 at
   // 14, 122.7 at 20; 16 heads: 161.7, 149.9, 142.1, 135.4.
   static constexpr int EXTRA_SOLO = 1, EXTRA = ROWS_ == 8 ? 14 : 20;
-  static constexpr int MIN_RUN = 4;                              // units a CTA takes at least
+  static constexpr int MIN_RUN = 8;                              // units a CTA takes at least
   static constexpr int NT = TOK / 8;                             // score tiles of 8 tokens
   static constexpr int KS = DP_ / 16;                            // inner steps of Q K^T
   static constexpr int OT = DP_ / 8;                             // output tiles of 8 columns
@@ -290,7 +290,7 @@ struct Loader {
     }
     page = -1;
     if (p.aligned || ((bits >> (lane % S::TOK)) & 1u & (lane < S::TOK)) != 0u)
-      page = __ldg(p.a.block_table + at.b * p.a.table_stride + column);
+      page = p.a.block_table[at.b * p.a.table_stride + column];
   }
   // Moves to the warp's next tile, through the shares that have none for it.
   __device__ __forceinline__ void prepare(const Params& p, int warp, int lane, int items) {

@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(VE == 1 ? kMaxThreads : kThreads, VE == 1 ? 1 
                                            : static_cast<const int*>(a.positions)[from];
     float c = __int_as_float(0x7fffffff), s = c;     // NaN
     if (p >= 0 && p < a.max_position) {
-      c = __ldg(a.cos_sin + p * a.rot + pair);
-      s = __ldg(a.cos_sin + p * a.rot + half + pair);
+      c = a.cos_sin[p * a.rot + pair];
+      s = a.cos_sin[p * a.rot + half + pair];
     } else if (a.status != nullptr) {
       atomicCAS(a.status, 0, DG_ERR_POSITION);
     }
@@ -256,7 +256,7 @@ __global__ void __launch_bounds__(VE == 1 ? kMaxThreads : kThreads, VE == 1 ? 1 
       if constexpr (std::is_same<C, E4m3>::value) {
         const float* scales = is_v ? a.v_scale : a.k_scale;
         if (scales != nullptr) {
-          const float scale = __ldg(scales + head);
+          const float scale = scales[head];
 #pragma unroll
           for (int j = 0; j < VE; ++j) {
             x[j] = x[j] / scale;
