@@ -99,12 +99,18 @@ struct Shape {
   static constexpr bool kE4m3 = E4M3_;
   static constexpr int DP = DP_, ROWS = ROWS_;
   static constexpr int ES = E4M3_ ? 1 : 2;
-  static constexpr int NW = DP_ == 64 ? 12 : DP_ == 128 ? 8 : 4; // warps
-  static constexpr int TOK = E4M3_ || DP_ == 64 ? 32 : 16;       // tokens a stage
+  // A stage holds a tile's keys and values.  With heads of 256 there is room
+  // for 4 warps' rings then, and for 8 if keys and values are stages of their
+  // own, half as much of them on its way: worth it where the products weigh
+  // more (ragged batch of 64 heads on 4, bf16: 281 -> 219 us; e4m3, 8 heads an
+  // item: 230 -> 202; but bf16, 4 heads an item: 144 -> 158).
+  static constexpr bool HALVES = DP_ == 256 && (E4M3_ || ROWS_ == 16);
+  static constexpr int NW = DP_ == 64 ? 12 : DP_ == 128 || HALVES ? 8 : 4;   // warps
+  static constexpr int TOK = E4M3_ || DP_ == 64 ? 32 : 16;       // tokens a tile
   static constexpr int STAGES = DP_ == 64 ? 2 : 3;
   static constexpr int PITCH = DP_ * ES;                         // bytes a row
-  static constexpr int KV_BYTES = TOK * PITCH;                   // a stage's keys; its values follow
-  static constexpr int STAGE = 2 * KV_BYTES;
+  static constexpr int KV_BYTES = TOK * PITCH;                   // a tile's keys, and its values
+  static constexpr int STAGE = HALVES ? KV_BYTES : 2 * KV_BYTES;
   static constexpr int RING = NW * STAGES * STAGE;
   static constexpr int JOIN = 8192;                              // floats of the join's buffer (32 KiB)
   static constexpr int JOIN_COLS =                               // columns a round: a power of two from 32
@@ -308,8 +314,10 @@ struct Loader {
     look_up(p, lane);
     tile += at.step();
   }
-  // Copies the pending tile into a stage.
+  // Copies the pending tile's keys, values or both into a stage.
+  template <bool KEYS, bool VALUES>
   __device__ __forceinline__ void issue(const Params& p, uint32_t stage, uint32_t* mask, int lane) const {
+    constexpr int kValuesAt = KEYS ? S::KV_BYTES : 0;
     if (!more) return;
     const dg_attention_args& a = p.a;
     const int chunk = lane % CH;
@@ -318,9 +326,9 @@ struct Loader {
     const uint32_t dst = stage + (lane / CH) * S::PITCH + S::swizzled(lane / CH, chunk) * 16;
     const bool good = page >= 0 && page < a.num_pages;
     if (p.aligned) {
-      if (!good && lane == 0) report(a.status, DG_ERR_PAGE);
+      if (KEYS && !good && lane == 0) report(a.status, DG_ERR_PAGE);
       const uint32_t live = good ? bits : 0u;
-      if (lane == 0) *mask = live;
+      if (KEYS && lane == 0) *mask = live;
       const char* k = keys + (page * a.k_cache_stride[0] + offset * a.k_cache_stride[1]) * S::ES;
       const char* v = values + (page * a.v_cache_stride[0] + offset * a.v_cache_stride[1]) * S::ES;
       const long long k_step = a.k_cache_stride[1] * (RPI * S::ES), v_step = a.v_cache_stride[1] * (RPI * S::ES);
@@ -329,8 +337,8 @@ struct Loader {
         for (int i = 0; i < S::TOK / RPI; ++i, k += k_step, v += v_step) {
           const uint32_t to = (dst ^ (S::swizzled(i * RPI, 0) * 16)) + i * RPI * S::PITCH;
           if (wanted) {
-            dg::warp::cp_async16(to, k);
-            dg::warp::cp_async16(to + S::KV_BYTES, v);
+            if (KEYS) dg::warp::cp_async16(to, k);
+            if (VALUES) dg::warp::cp_async16(to + kValuesAt, v);
           }
         }
       } else {
@@ -344,17 +352,17 @@ struct Loader {
           const uint32_t to = (dst ^ (S::swizzled(i * RPI, 0) * 16)) + i * RPI * S::PITCH;
           const uint32_t bytes = (live >> (i * RPI + lane / CH)) & 1u ? 16u : 0u;
           if (wanted) {
-            dg::warp::cp_async16(to, k, bytes);
-            dg::warp::cp_async16(to + S::KV_BYTES, v, bytes);
+            if (KEYS) dg::warp::cp_async16(to, k, bytes);
+            if (VALUES) dg::warp::cp_async16(to + kValuesAt, v, bytes);
           }
         }
       }
       return;
     }
     const bool seen = lane < S::TOK && ((bits >> (lane % S::TOK)) & 1u) != 0u;
-    if (seen && !good) report(a.status, DG_ERR_PAGE);
+    if (KEYS && seen && !good) report(a.status, DG_ERR_PAGE);
     const uint32_t live = __ballot_sync(0xffffffffu, seen && good);
-    if (lane == 0) *mask = live;
+    if (KEYS && lane == 0) *mask = live;
     long long k_at = 0, v_at = 0;
     if (seen && good) {
       k_at = (page * a.k_cache_stride[0] + offset * a.k_cache_stride[1]) * S::ES;
@@ -368,8 +376,8 @@ struct Loader {
       const uint32_t bytes = (live >> r) & 1u ? 16u : 0u;
       const uint32_t to = (dst ^ (S::swizzled(i * RPI, 0) * 16)) + i * RPI * S::PITCH;
       if (wanted) {
-        dg::warp::cp_async16(to, keys + kr + (bytes ? chunk * 16 : 0), bytes);
-        dg::warp::cp_async16(to + S::KV_BYTES, values + vr + (bytes ? chunk * 16 : 0), bytes);
+        if (KEYS) dg::warp::cp_async16(to, keys + kr + (bytes ? chunk * 16 : 0), bytes);
+        if (VALUES) dg::warp::cp_async16(to + kValuesAt, values + vr + (bytes ? chunk * 16 : 0), bytes);
       }
     }
   }
@@ -469,11 +477,11 @@ struct Warp {
     }
   }
 
-  // One stage: TOK tokens, of which `live` are to be seen.
-  __device__ __forceinline__ void step(const Params& p, uint32_t keys, uint32_t live, int lane) {
-    const uint32_t values = keys + S::KV_BYTES;
+  // One tile, of whose TOK tokens `live` are to be seen: its probabilities s
+  // (to the reference exponent m, which may move), then their part of o.
+  __device__ __forceinline__ void scores(const Params& p, uint32_t keys, uint32_t live, int lane,
+                                         float (&s)[S::NT][4]) {
     const int g = lane >> 2, quad = lane & 3;
-    float s[S::NT][4];
 #pragma unroll
     for (int t = 0; t < S::NT; ++t)
 #pragma unroll
@@ -579,7 +587,10 @@ struct Warp {
         o[t][3] *= alpha[R - 1];
       }
     }
+  }
 
+  __device__ __forceinline__ void weigh(uint32_t values, int lane, const float (&s)[S::NT][4]) {
+    const int g = lane >> 2, quad = lane & 3;
 #pragma unroll
     for (int kk = 0; kk < S::NT / 2; ++kk) {
       // hi and lo of the probabilities of 16 tokens as the first operand.
@@ -884,15 +895,24 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
   const uint32_t ring = dg::sm100::smem_addr(smem) + warp * (S::STAGES * S::STAGE);
   uint32_t* mask = masks + warp * S::STAGES;
   loader.prepare(p, warp, lane, items);
-#pragma unroll
-  for (int i = 0; i < S::STAGES - 1; ++i) {
-    loader.issue(p, ring + i * S::STAGE, mask + i, lane);
+  if constexpr (S::HALVES) {
+    loader.template issue<true, false>(p, ring, mask, lane);
+    dg::warp::cp_async_commit();
+    loader.template issue<false, true>(p, ring + S::STAGE, mask, lane);
     dg::warp::cp_async_commit();
     loader.prepare(p, warp, lane, items);
+  } else {
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) {
+      loader.template issue<true, true>(p, ring + i * S::STAGE, mask + i, lane);
+      dg::warp::cp_async_commit();
+      loader.prepare(p, warp, lane, items);
+    }
   }
 
   Warp<S> w;
-  int stage = 0;
+  int stage = 0;                            // of the tile (of its keys)
+  int turn = 0;                             // tiles so far, modulo 2
   bool mine_too = run && (!at.solo || at.first_tile(warp) == 0);
   if (mine_too) w.fetch(p, at.b, at.item, lane);
   while (run) {
@@ -902,14 +922,33 @@ __global__ void __launch_bounds__(S::NW * 32, 1) attention_kernel(const __grid_c
       w.begin(p, share.item);
       const int step = share.step();
       for (int tile = share.first_tile(warp); tile < share.count; tile += step) {
+        float s[S::NT][4];
         dg::warp::cp_async_wait<S::STAGES - 2>();
         __syncwarp();      // every lane's copies of this stage landed, every lane is done with the one before
-        const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
-        loader.issue(p, ring + ahead * S::STAGE, mask + ahead, lane);
-        dg::warp::cp_async_commit();
-        loader.prepare(p, warp, lane, items);
-        w.step(p, ring + stage * S::STAGE, mask[stage], lane);
-        stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+        if constexpr (S::HALVES) {
+          // Stages in turn: keys, values, the next tile's keys.
+          const int values = stage == 2 ? 0 : stage + 1, next = values == 2 ? 0 : values + 1;
+          loader.template issue<true, false>(p, ring + next * S::STAGE, mask + (turn ^ 1), lane);
+          dg::warp::cp_async_commit();
+          w.scores(p, ring + stage * S::STAGE, mask[turn], lane, s);
+          dg::warp::cp_async_wait<S::STAGES - 2>();
+          __syncwarp();
+          loader.template issue<false, true>(p, ring + stage * S::STAGE, mask, lane);
+          dg::warp::cp_async_commit();
+          loader.prepare(p, warp, lane, items);
+          w.weigh(ring + values * S::STAGE, lane, s);
+          stage = next;
+          turn ^= 1;
+        } else {
+          const int ahead = stage == 0 ? S::STAGES - 1 : stage - 1;
+          const uint32_t from = ring + stage * S::STAGE;
+          loader.template issue<true, true>(p, ring + ahead * S::STAGE, mask + ahead, lane);
+          dg::warp::cp_async_commit();
+          loader.prepare(p, warp, lane, items);
+          w.scores(p, from, mask[stage], lane, s);
+          w.weigh(from + S::KV_BYTES, lane, s);
+          stage = stage == S::STAGES - 1 ? 0 : stage + 1;
+        }
       }
     }
     // The next share's q is on its way during the join.
