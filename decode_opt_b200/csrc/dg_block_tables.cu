@@ -17,8 +17,10 @@
 // for the table entry that the same launch writes: a page below ceil(c / P) is
 // read from the table, a later one from the free list itself.
 //
-// Bound: a handful of dependent loads for a decode step (latency), the 16
-// bytes a token at the other end.
+// Bound: the launch, three dependent loads and the scan for a decode step
+// (B200, in a graph: 4.4 us for 16 requests, 5.8 for 512); the searches'
+// instructions at the other end (4096 prompts, 1.4 million tokens, 23 MB:
+// 16 us, where the bytes alone would take 3.6).
 
 #include <cuda_runtime.h>
 
