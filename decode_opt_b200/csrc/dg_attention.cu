@@ -611,9 +611,12 @@ struct Warp {
           const uint32_t top = S::MM::cut(u, v);
           const float2 back = S::MM::unpack(top);
           hi[h * R + r] = top;
-          // (e4m3 has no infinity to keep)
+          // (e4m3 has no infinity to keep; a probability below kTiny is itself:
+          // with kTiny, 2^-34 of the largest in fp16, 100,000 tokens of no
+          // weight added 2^-17 of their values)
           lo[h * R + r] = S::kE4m3 ? S::MM::pack(u - back.x, v - back.y)
-                                   : S::MM::pack(fmaxf(u - back.x, S::MM::kTiny), fmaxf(v - back.y, S::MM::kTiny));
+                                   : S::MM::pack(fmaxf(u - back.x, fminf(u, S::MM::kTiny)),
+                                                 fmaxf(v - back.y, fminf(v, S::MM::kTiny)));
         }
       uint32_t x[4], y[4];
       if constexpr (R == 1) {
