@@ -80,6 +80,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFp8Max = 448.0f;        // of the output's quantisation, as dg_quantize_act
 constexpr float kQuantEps = 1.0e-4f;
 constexpr float kNegInf = -__builtin_huge_valf();
+constexpr float kLowest = -3.402823466e38f;
 
 // Workspace: tickets, then (m, l) per share and row, then the shares.
 constexpr size_t kTicketBytes = 1024;    // kMaxCtas ints
@@ -568,6 +569,9 @@ struct Warp {
         for (int i = 0; i < 2; ++i) top = fmaxf(top, s[t][2 * r + i]);
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // -inf stands for "no token so far" alone: a row whose scores are -inf
+      // or NaN has seen some.
+      top = live != 0u ? fmaxf(top, kLowest) : kNegInf;
       alpha[r] = 1.0f;
       if (top > m[r] + S::kLag || m[r] == kNegInf) {
         moved = moved || m[r] != kNegInf;
