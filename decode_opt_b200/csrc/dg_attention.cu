@@ -715,6 +715,10 @@ __device__ __forceinline__ void load_pack(const float* from, float (&x)[N]) {
   }
 }
 
+// What a finished row is multiplied with.  None of its tokens may have been
+// seen (bad pages): it is 0 then, as where there are none.
+__device__ __forceinline__ float inverse_sum(float m, float l) { return m == kNegInf ? 0.0f : 1.0f / l; }
+
 // A finished row: this lane's column of each 32-column chunk, unnormalised.
 template <typename S>
 __device__ __forceinline__ void finish_row(const Params& p, int b, int item, int row, const float (&v)[S::CHUNKS],
@@ -724,7 +728,7 @@ __device__ __forceinline__ void finish_row(const Params& p, int b, int item, int
   const int in_group = (item - head * p.groups) * S::ROWS + row;
   if (in_group >= p.group) return;
   const int h = head * p.group + in_group;
-  float norm = 1.0f / l;
+  float norm = inverse_sum(m, l);
   if (S::kE4m3 && a.v_scale != nullptr) norm *= a.v_scale[head];
   const long long at = b * a.out_stride[0] + h * a.out_stride[1];
 #pragma unroll
@@ -778,7 +782,7 @@ __device__ __forceinline__ void finish_solo(const Params& p, int b, int item, co
     const int in_group = (item - head * p.groups) * S::ROWS + g + 8 * r;
     const bool real = in_group < p.group;
     const int h = head * p.group + in_group;
-    float norm = 1.0f / l;
+    float norm = inverse_sum(w.m[r], l);
     if (S::kE4m3 && a.v_scale != nullptr) norm *= a.v_scale[head];
     const long long at = b * a.out_stride[0] + h * a.out_stride[1];
     if (real && a.lse != nullptr && quad == 0)
