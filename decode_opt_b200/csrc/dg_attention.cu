@@ -397,6 +397,24 @@ __device__ __forceinline__ float2 unpack_q(uint32_t v, int type) {
   return type == DG_TYPE_BF16 ? Bf16::unpack(v) : Fp16::unpack(v);
 }
 
+// cap * tanh(x).  Up to kNearCap: x + x^3 p(x^2), p of the least relative error
+// that its degree allows there (found by Remez exchange: 2^-26; with its
+// roundings 2^-23).  Beyond, 1 - 2 / (e^(2x) + 1) no longer cancels: 2^-21.
+// The second alone, for all, is off by 2^-23 of the cap, not of the score.  Most
+// heads' scores stay below half the cap, and their warps take the first alone.
+// (33 requests of 24 fp16 heads 63.5 -> 64.3 us, e4m3 with 16 heads an item
+// 237 -> 246; tanhf() in place of both 64.8 and 264.)
+constexpr float kNearCap = 0.5f;
+__device__ __forceinline__ float capped_near(float x, float cap) {
+  const float t = x * x;
+  const float p = fmaf(fmaf(fmaf(0.0172414915f, t, -0.0530454943f), t, 0.133258790f), t, -0.333331439f);
+  const float u = cap * x;
+  return fmaf(u * t, p, u);
+}
+__device__ __forceinline__ float capped_far(float x, float cap) {
+  return cap - 2.0f * cap * dg::warp::rcp_approx(dg::warp::exp2_approx(x * (2.0f * kLog2e)) + 1.0f);
+}
+
 // One warp's state for one item.
 template <typename S>
 struct Warp {
@@ -404,7 +422,7 @@ struct Warp {
   uint32_t q[S::KS][2 * R];                          // [step][first half's rows, second half's rows]
   float o[S::OT][4];
   float m[R], l[R];
-  float factor[R];                                   // score -> exponent of 2 (capped: of the tanh's exponential)
+  float factor[R];                                   // score -> exponent of 2 (capped: -> score over the cap)
 
   // Loads an item's q as it lies in memory; nothing waits for it before
   // begin().
@@ -462,7 +480,7 @@ struct Warp {
         f *= up;
         if (a.k_scale != nullptr) f *= a.k_scale[p.groups == 1 ? item : item / p.groups];
       }
-      factor[r] = a.softcap > 0.0f ? 2.0f * kLog2e * (f / a.softcap) : f * kLog2e;
+      factor[r] = a.softcap > 0.0f ? f / a.softcap : f * kLog2e;
       m[r] = kNegInf;
       l[r] = 0.0f;
     }
@@ -540,13 +558,24 @@ struct Warp {
 #pragma unroll
       for (int i = 0; i < 2 * R; ++i) s[t][i] *= factor[i >> 1];
     if (capped) {
-      // tanh(x) = 1 - 2 / (e^(2x) + 1): off by about 2^-22, as the score that
-      // it is a part of (cap = softcap * log2 e, factor has 2 log2 e).
+      // Here s is the score over the cap.
+      float top = 0.0f;
 #pragma unroll
       for (int t = 0; t < S::NT; ++t)
 #pragma unroll
-        for (int i = 0; i < 2 * R; ++i)
-          s[t][i] = cap - 2.0f * cap * dg::warp::rcp_approx(dg::warp::exp2_approx(s[t][i]) + 1.0f);
+        for (int i = 0; i < 2 * R; ++i) top = fmaxf(top, fabsf(s[t][i]));
+      if (__any_sync(0xffffffffu, top > kNearCap)) {
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2 * R; ++i)
+            s[t][i] = fabsf(s[t][i]) > kNearCap ? capped_far(s[t][i], cap) : capped_near(s[t][i], cap);
+      } else {
+#pragma unroll
+        for (int t = 0; t < S::NT; ++t)
+#pragma unroll
+          for (int i = 0; i < 2 * R; ++i) s[t][i] = capped_near(s[t][i], cap);
+      }
     }
     if (live != Loader<S>::kWhole) {
 #pragma unroll
@@ -1204,6 +1233,10 @@ int dg_paged_attention(const dg_attention_args* args, void* stream, int pdl_attr
   if (args == nullptr || refused(*args)) return cudaErrorInvalidValue;
   Params p{};
   p.a = *args;
+  // Caps below 2^-100 leave nothing of a score and those above take nothing
+  // from it; in between their quotients and products stay finite.
+  if (p.a.softcap > 0.0f)
+    p.a.softcap = p.a.softcap < 0x1p-100f ? 0x1p-100f : p.a.softcap > 0x1p100f ? 0x1p100f : p.a.softcap;
   p.group = p.a.heads / p.a.kv_heads;
   Entry& e = pick(p.a, p.group <= 8);
   p.groups = (p.group + e.rows - 1) / e.rows;
