@@ -78,11 +78,16 @@ class DecodeAttention:
         self.w_qkv = dg.prepack_weight(w_qkv, self.qkv_config.packed_rows, layout)
         self.w_out = dg.prepack_weight(w_out, self.out_config.packed_rows, layout)
         self.qkv_scales, self.out_scales = qkv_scales, out_scales
-        self.workspace = dg.attention_workspace(w_qkv.device)
 
-    def step(self, x, step: "dg.StepTables", block_table, cache: PagedCache, table) -> torch.Tensor:
-        """One token of each request: x [M, hidden] bf16 -> [M, hidden] bf16.
-        `step` is of the same M requests, one new token each, without padding."""
+    def step(self, x, step: "dg.StepTables", block_table, cache: PagedCache, table, workspace=None) -> torch.Tensor:
+        """One token of each request: x [M, hidden] bf16 -> [M, hidden] bf16, on
+        the current stream.  `step` is of the same M requests, one new token
+        each, without padding.
+
+        Steps may run on several streams at once.  `workspace` is that of
+        :func:`dg.paged_attention`: by default its own per stream and per
+        captured call.  One from :func:`dg.attention_workspace` saves a captured
+        step the zeroing; steps that share it must not overlap."""
         s, m = self.shape, x.shape[0]
         act, act_scales = dg.quantize_activation(x, stream=torch.cuda.current_stream(x.device))
         qkv = dg.fp8_decode_gemm(act, act_scales, self.w_qkv, self.qkv_scales, config=self.qkv_config, n=s.qkv_width)
@@ -90,7 +95,7 @@ class DecodeAttention:
         q, k, v = qkv.split_with_sizes((s.heads, s.kv_heads, s.kv_heads), 1)
         q = dg.rotary_append(q, k, v, step.positions, step.slots, cache.k, cache.v, table, sections=s.sections,
                              k_scale=cache.k_scale, v_scale=cache.v_scale)
-        kw = dict(window=s.window, k_scale=cache.k_scale, v_scale=cache.v_scale, workspace=self.workspace)
+        kw = dict(window=s.window, k_scale=cache.k_scale, v_scale=cache.v_scale, workspace=workspace)
         if s.head_dim % 128 == 0:
             act = torch.empty((m, s.q_width), dtype=torch.uint8, device=x.device)
             act_scales = torch.empty((m, s.q_width // 128), dtype=torch.float32, device=x.device)
@@ -141,10 +146,11 @@ def main(argv=None) -> int:
     lens = torch.full((m,), o.context, dtype=torch.int32, device=dev)
     new = torch.ones(m, dtype=torch.int32, device=dev)
     x = torch.randn(m, o.hidden, device=dev).bfloat16()
+    workspace = dg.attention_workspace(dev)
 
     def once():
         t = dg.build_block_tables(lens, new, free, block_table, o.page_size, m, cursor=cursor)
-        y = layer.step(x, t, block_table, cache, table)
+        y = layer.step(x, t, block_table, cache, table, workspace)
         x.copy_(y)
         lens.copy_(t.seq_lens)
         cursor.copy_(t.cursor)
