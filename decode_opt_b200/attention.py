@@ -267,8 +267,9 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: Option
     `q_out` (uint8 [B, Hq * D]) and `q_scales` (fp32 [B, Hq * D / 128]) also
     receive the result quantised for the next product, the bytes of
     ``quantize_activation`` (bf16 and D a multiple of 128).  `workspace`: from
-    :func:`attention_workspace`; by default one is kept per stream, and a call
-    under capture gets its own, zeroed in the graph."""
+    :func:`attention_workspace`; by default one is kept per stream (and host
+    thread, on the per-thread default stream), and a call under capture gets
+    its own, zeroed in the graph."""
     if stream is not None:
         with _on(q, stream):
             return paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale=scale, window=window,

@@ -21,6 +21,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -28,6 +29,7 @@
 #include <map>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <utility>
 
 #include "decode_attention_b200.h"
@@ -411,7 +413,15 @@ Tensor new_workspace(c10::Device device) {
   return ws;
 }
 
-// Kept per stream: calls on one stream run one after another.  A captured
+// A number for each host thread that asks, never given twice.
+int64_t thread_number() {
+  static std::atomic<int64_t> next{1};
+  thread_local const int64_t mine = next++;
+  return mine;
+}
+
+// Kept per stream: calls on one stream run one after another.  The per-thread
+// default stream's handle names another stream in each host thread.  A captured
 // graph may be replayed on any stream, so it gets its own, from its pool.
 Tensor stream_workspace(c10::Device device, void* stream) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
@@ -419,8 +429,8 @@ Tensor stream_workspace(c10::Device device, void* stream) {
       capture != cudaStreamCaptureStatusNone)
     return new_workspace(device);
   // (never destroyed: the process's end is no time to call the GPU's allocator)
-  static auto* kept = new std::map<std::pair<int, void*>, Tensor>();
-  Tensor& ws = (*kept)[{device.index(), stream}];
+  static auto* kept = new std::map<std::tuple<int, void*, int64_t>, Tensor>();
+  Tensor& ws = (*kept)[{device.index(), stream, stream == cudaStreamPerThread ? thread_number() : 0}];
   if (!ws.defined()) ws = new_workspace(device);
   return ws;
 }
