@@ -117,6 +117,12 @@ def random_layer(shape: LayerShape, batch: int, seed: int = 0, device="cuda") ->
     return DecodeAttention(shape, *weight(shape.qkv_width, shape.hidden), *weight(shape.hidden, shape.q_width), batch)
 
 
+def free_list(block_table, held: int):
+    """The pages of the table's columns from `held` on, as a free list of its
+    own: a view of the table would be overwritten as the table is filled."""
+    return block_table[:, held:].flatten().clone()
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     ap.add_argument("--requests", type=int, default=32)
@@ -139,7 +145,7 @@ def main(argv=None) -> int:
     held = -(-o.context // o.page_size)
     pool = torch.randperm(m * width, device=dev).to(torch.int32)
     block_table = pool.view(m, width).clone()
-    free, cursor = block_table[:, held:].contiguous().view(-1), torch.zeros(1, dtype=torch.int32, device=dev)
+    free, cursor = free_list(block_table, held), torch.zeros(1, dtype=torch.int32, device=dev)
     scales = [torch.full((o.kv_heads,), 0.02, device=dev) if o.e4m3_cache else None for _ in range(2)]
     cache = PagedCache(shape, m * width, o.page_size, torch.float8_e4m3fn if o.e4m3_cache else torch.bfloat16, *scales)
     table = dg.rope_table(o.context + o.steps + 8, o.head_dim)
