@@ -255,6 +255,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
+// Whether the free list lies in a row of the table: a launch reads the one and
+// writes the other in no order.
+bool free_list_in_table(const dg_block_tables& a) {
+  const uintptr_t from = reinterpret_cast<uintptr_t>(a.free_pages), to = from + 4ull * a.free_count;
+  const uintptr_t table = reinterpret_cast<uintptr_t>(a.block_table);
+  const unsigned long long row = 4ull * a.table_width, step = 4ull * a.table_stride;
+  // The first row that ends past the list's beginning.
+  const unsigned long long b = from < table + row ? 0 : (from - table - row) / step + 1;
+  return a.free_count > 0 && b < static_cast<unsigned long long>(a.batch) && table + b * step < to;
+}
+
 }  // namespace
 
 extern "C" int dg_build_block_tables(const dg_block_tables* args, void* stream, int pdl_attr) {
@@ -271,6 +282,7 @@ extern "C" int dg_build_block_tables(const dg_block_tables* args, void* stream, 
   // Other CTAs read these while CTA 0 writes.
   if (a.seq_lens == a.context_lens || a.seq_lens == a.new_lens || a.cursor_out == a.cursor_in)
     return cudaErrorInvalidValue;
+  if (free_list_in_table(a)) return cudaErrorInvalidValue;
 
   const size_t smem = static_cast<size_t>((a.batch + 4) & ~3) * 3 * sizeof(int);
   // A token a thread; past the CTAs that fit at once a CTA takes several

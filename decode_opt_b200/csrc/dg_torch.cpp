@@ -126,6 +126,15 @@ std::pair<int, int64_t> table_of(const Tensor& t, int64_t batch, c10::Device dev
   return {static_cast<int>(t.size(1)), batch > 1 ? t.stride(0) : t.size(1)};
 }
 
+// Whether part of the vector lies in one of the rows.
+bool in_rows(const int* vector, int64_t count, const int* rows, int64_t batch, int64_t width, int64_t stride) {
+  const auto from = reinterpret_cast<uintptr_t>(vector), to = from + 4 * static_cast<uintptr_t>(count);
+  const auto first = reinterpret_cast<uintptr_t>(rows), row = 4 * static_cast<uintptr_t>(width);
+  const auto step = 4 * static_cast<uintptr_t>(stride);
+  const uintptr_t b = from < first + row ? 0 : (from - first - row) / step + 1;    // the first that ends past `from`
+  return count > 0 && b < static_cast<uintptr_t>(batch) && first + b * step < to;
+}
+
 int type_of(at::ScalarType t) {
   switch (t) {
     case at::kBFloat16: return DG_TYPE_BF16;
@@ -240,6 +249,8 @@ PyObject* build_block_tables(PyObject*, PyObject* const* arg, Py_ssize_t count) 
       a.cursor_in = data<int>(t);
     }
     a.block_table = data<int>(table);
+    need(!in_rows(a.free_pages, a.free_count, a.block_table, batch, width, table_stride),
+         "free_pages must not be part of block_table");
     a.status = status_of(arg[8], device);
     const c10::cuda::CUDAGuard guard(device);
     Tensor made[6];

@@ -67,7 +67,7 @@ typedef struct dg_block_tables {
   long long table_stride;    /* elements between rows of block_table, >= table_width             */
   const int* context_lens;   /* [batch]                                                          */
   const int* new_lens;       /* [batch]                                                          */
-  const int* free_pages;     /* [free_count]                                                     */
+  const int* free_pages;     /* [free_count]; no part of block_table                             */
   const int* cursor_in;      /* [1], may be NULL                                                 */
   int* block_table;          /* [batch, table_width]                                             */
   int* seq_lens;             /* [batch]; not context_lens or new_lens                            */

@@ -65,3 +65,18 @@ def test_a_stream_keeps_its_workspace():
         t.join()
         torch.cuda.synchronize()
         assert torch.cuda.memory_allocated() == before
+
+
+def test_a_free_list_inside_the_block_table_is_refused():
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    new = torch.ones_like(lens)
+    wide = torch.arange(30, dtype=torch.int32, device="cuda").view(3, 10)
+    table = wide[:, :6]
+    for free in (wide.view(-1), wide[0, 5:7], wide[1, 3:4], wide.view(-1)[8:21]):
+        with pytest.raises(ValueError):
+            dg.build_block_tables(lens, new, free, table, 4, 3)
+    # Beside the rows it is a list like any other.
+    got = dg.build_block_tables(lens, new, wide[0, 6:], table, 4, 3)
+    assert table[:, 0].tolist() == [6, 7, 8] and got.cursor.tolist() == [3]
+    got = dg.build_block_tables(lens, new, wide[2, 7:], table, 4, 3)
+    assert table[:, 0].tolist() == [27, 28, 29] and got.slots.tolist() == [108, 112, 116]
