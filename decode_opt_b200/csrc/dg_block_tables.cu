@@ -24,6 +24,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <climits>
 #include <cstdint>
 
@@ -255,6 +256,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 }
 
+// The kernel's three arrays.
+constexpr size_t smem_of(int batch) { return static_cast<size_t>((batch + 4) & ~3) * 3 * sizeof(int); }
+constexpr size_t kPlainSmem = 48 * 1024;     // what a kernel may take without asking
+static_assert(smem_of(kMaxBatch) <= 227 * 1024 - 1024, "shared memory");
+
 // Whether the free list lies in a row of the table: a launch reads the one and
 // writes the other in no order.
 bool free_list_in_table(const dg_block_tables& a) {
@@ -284,7 +290,7 @@ extern "C" int dg_build_block_tables(const dg_block_tables* args, void* stream, 
     return cudaErrorInvalidValue;
   if (free_list_in_table(a)) return cudaErrorInvalidValue;
 
-  const size_t smem = static_cast<size_t>((a.batch + 4) & ~3) * 3 * sizeof(int);
+  const size_t smem = smem_of(a.batch);
   // A token a thread; past the CTAs that fit at once a CTA takes several
   // rounds rather than the sums being made again.
   const int sms = dg_num_sms() > 0 ? dg_num_sms() : 148;
@@ -294,10 +300,20 @@ extern "C" int dg_build_block_tables(const dg_block_tables* args, void* stream, 
   int shift = -1;
   if ((a.page_size & (a.page_size - 1)) == 0)
     for (shift = 0; (1 << shift) < a.page_size; ++shift) {}
-  if (smem > 48 * 1024) {
-    const cudaError_t err = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(smem));
+  if (smem > kPlainSmem) {
+    // Raised once per device, to what the largest batch takes: it is the
+    // kernel's, not the call's, and another thread may be about to launch.
+    static std::atomic<unsigned long long> ready{0};
+    int dev = 0;
+    cudaError_t err = cudaGetDevice(&dev);
     if (err != cudaSuccess) return err;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if ((ready.load(std::memory_order_acquire) & bit) == 0) {
+      err = cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 static_cast<int>(smem_of(kMaxBatch)));
+      if (err != cudaSuccess) return err;
+      ready.fetch_or(bit, std::memory_order_release);
+    }
   }
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[1]{};
