@@ -258,8 +258,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 // The kernel's three arrays.
 constexpr size_t smem_of(int batch) { return static_cast<size_t>((batch + 4) & ~3) * 3 * sizeof(int); }
-constexpr size_t kPlainSmem = 48 * 1024;     // what a kernel may take without asking
-static_assert(smem_of(kMaxBatch) <= 227 * 1024 - 1024, "shared memory");
+constexpr size_t kStaticSmem = sizeof(Sums) * 2 * kWarps;          // of the kernel's own, beside them
+constexpr size_t kPlainSmem = 48 * 1024 - kStaticSmem;             // what it may take without asking
+static_assert(smem_of(kMaxBatch) + kStaticSmem <= 227 * 1024 - 1024, "shared memory");
 
 // Whether the free list lies in a row of the table: a launch reads the one and
 // writes the other in no order.
