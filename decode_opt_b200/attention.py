@@ -17,8 +17,8 @@ ValueError before anything is launched.  What only the GPU can see (lengths,
 pages, slots, positions) is checked there: the access is left out and `status`,
 an optional zeroed int32 tensor, receives a code (:func:`status_string`).
 Nothing synchronises; every call can be captured in a CUDA graph.  Only
-:func:`rotary` has a gradient.  `stream`
-(default: the current one) takes a torch stream or a cudaStream_t handle;
+:func:`rotary` has a gradient, in q and k: a tensor that wants one elsewhere
+raises ValueError.  `stream` (default: the current one) takes a torch stream or a cudaStream_t handle;
 outputs made here are allocated on it.
 """
 
@@ -207,6 +207,8 @@ def rotary(q, k, positions, table, *, sections: Optional[Sequence[int]] = None, 
     if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
         if out_q is not None or out_k is not None:
             raise ValueError("out_q and out_k do not go with a gradient")
+        if table.requires_grad:
+            raise ValueError("the table has no gradient")
         return _Rotary.apply(q, k, positions, table, pairs, inverse, status, pdl_attr)
     return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
                         out_q if out_q is not None else (q is not None or None),

@@ -97,8 +97,10 @@ P* data(const Tensor& t) {
   return static_cast<P*>(t.data_ptr());
 }
 
-void no_gradient(const Tensor& t, const char* call) {
-  need(!(t.requires_grad() && c10::GradMode::is_enabled()), "%s has no gradient: call it under torch.no_grad()", call);
+// An argument, read or written, that wants a gradient where the call has none.
+void no_gradient(PyObject* o, const char* call) {
+  if (!THPVariable_Check(o) || !c10::GradMode::is_enabled()) return;
+  need(!THPVariable_Unpack(o).requires_grad(), "%s has no gradient for one of its tensors that wants one: call it under torch.no_grad()", call);
 }
 
 // A contiguous vector of `count` values.
@@ -338,6 +340,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     a.max_position = static_cast<int>(table.size(0));
     a.rot = static_cast<int>(table.size(1));
     a.cos_sin = data<float>(table);
+    for (int i : {7, 14, 15}) no_gradient(arg[i], "rotary");
     const int64_t axes = whole(arg[8], "axes");
     need(PyBytes_Check(arg[9]) && PyBytes_GET_SIZE(arg[9]) == static_cast<Py_ssize_t>(sizeof(a.axis_of)),
          "words must be the packed axes");
@@ -362,9 +365,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     if (given(arg[5])) {
       need(q != nullptr && k != nullptr, "the cache write takes q, k and v");
       const Tensor& v = tensor(arg[2], "v");
-      no_gradient(*q, "rotary_append");
-      no_gradient(*k, "rotary_append");
-      no_gradient(v, "rotary_append");
+      for (int i : {0, 1, 2, 5, 6, 12, 13}) no_gradient(arg[i], "rotary_append");
       need(kind != DG_TYPE_FP32, "the cache write takes bf16 or fp16");
       need(heads_of(v, "v", x, a.v_stride) == a.kv_heads,
            "k and v must have one shape");
@@ -460,7 +461,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     const int kind = type_of(q.scalar_type());
     need(q.is_cuda() && q.dim() == 3 && (kind == DG_TYPE_BF16 || kind == DG_TYPE_FP16),
          "q must be a bf16 or fp16 CUDA tensor [batch, heads, dim]");
-    no_gradient(q, "paged_attention");
+    for (int i : {0, 1, 2, 8, 9, 10, 12, 13}) no_gradient(arg[i], "paged_attention");
     const c10::Device device = q.device();
     const int64_t batch = q.size(0), heads = q.size(1), dim = q.size(2);
     need(batch >= 1 && batch <= kInt32Max && heads <= kInt32Max && q.stride(2) == 1 && q.stride(0) % 2 == 0 &&

@@ -1,0 +1,57 @@
+"""GPU tests of what autograd sees of the attention operators."""
+
+import pytest
+import torch
+
+import decode_opt_b200 as dg
+
+pytestmark = pytest.mark.gpu
+
+
+def _rotary_inputs(dtype=torch.float32):
+    g = torch.Generator(device="cuda").manual_seed(2)
+    q = torch.randn(5, 4, 32, generator=g, device="cuda").to(dtype)
+    k = torch.randn(5, 2, 32, generator=g, device="cuda").to(dtype)
+    return q, k, torch.arange(3, 8, device="cuda"), dg.rope_table(16, 16)
+
+
+def _attention_inputs():
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(2, 4, 128, generator=g, device="cuda").bfloat16()
+    k, v = (torch.randn(4, 8, 2, 128, generator=g, device="cuda").bfloat16() for _ in range(2))
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
+    return q, k, v, table, torch.tensor([5, 16], dtype=torch.int32, device="cuda")
+
+
+def test_tensors_that_want_a_gradient_and_get_none_are_refused():
+    q, kc, vc, table, lens = _attention_inputs()
+    f8 = kc.to(torch.float8_e4m3fn)
+    scale = torch.ones(2, device="cuda")
+    wants = lambda t: t.clone().requires_grad_()  # noqa: E731
+    for args, kw in (((wants(q), kc, vc), {}), ((q, wants(kc), vc), {}), ((q, kc, wants(vc)), {}),
+                     ((q, f8, f8), dict(k_scale=wants(scale))), ((q, f8, f8), dict(v_scale=wants(scale))),
+                     ((q, kc, vc), dict(out=wants(q))),
+                     ((q, kc, vc), dict(q_out=torch.empty(2, 512, dtype=torch.uint8, device="cuda"),
+                                        q_scales=wants(torch.ones(2, 4, device="cuda"))))):
+        with pytest.raises(ValueError):
+            dg.paged_attention(*args, table, lens, **kw)
+        with torch.no_grad():
+            dg.paged_attention(*args, table, lens, **kw)
+    x, k, pos, rope = _rotary_inputs(torch.bfloat16)
+    slots = torch.arange(5, device="cuda")
+    cache = torch.zeros(2, 4, 2, 32, device="cuda", dtype=torch.bfloat16)
+    c8, ones = cache.to(torch.float8_e4m3fn), torch.ones(2, device="cuda")
+    for args, kw in (((wants(x), k, k, pos, slots, cache, cache.clone(), rope), {}),
+                     ((x, k, k, pos, slots, wants(cache), cache.clone(), rope), {}),
+                     ((x, k, k, pos, slots, cache, wants(cache), rope), {}),
+                     ((x, k, k, pos, slots, cache, cache.clone(), wants(rope)), {}),
+                     ((x, k, k, pos, slots, c8, c8.clone(), rope), dict(k_scale=wants(ones))),
+                     ((x, k, k, pos, slots, cache, cache.clone(), rope), dict(out_q=wants(x)))):
+        with pytest.raises(ValueError):
+            dg.rotary_append(*args, **kw)
+        with torch.no_grad():
+            dg.rotary_append(*args, **kw)
+    for args, kw in (((x, k, pos, wants(rope)), {}), ((wants(x), k, pos, wants(rope)), {}),
+                     ((x, k, pos, rope), dict(out_q=wants(x))), ((x, k, pos, rope), dict(out_k=wants(k)))):
+        with pytest.raises(ValueError):
+            dg.rotary(*args, **kw)
