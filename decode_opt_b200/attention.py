@@ -18,8 +18,8 @@ pages, slots, positions) is checked there: the access is left out and `status`,
 an optional zeroed int32 tensor, receives a code (:func:`status_string`).
 Nothing synchronises; every call can be captured in a CUDA graph.  Only
 :func:`rotary` has a gradient, in q and k: a tensor that wants one elsewhere
-raises ValueError.  `stream` (default: the current one) takes a torch stream or a cudaStream_t handle;
-outputs made here are allocated on it.
+raises ValueError.  `stream` (default: the current one) takes a torch stream or
+a cudaStream_t handle; outputs made here are allocated on it.
 """
 
 from __future__ import annotations
@@ -34,6 +34,7 @@ from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -181,9 +182,33 @@ class _Rotary(torch.autograd.Function):
         dq, dk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
         gq = gk = None
         if dq is not None or dk is not None:
-            gq, gk = _host.rotary(dq, dk, None, positions, None, None, None, table, *ctx.pairs, not ctx.inverse, None,
-                                  None, dq is not None or None, dk is not None or None, None, False)
+            gq, gk = _rotated(dq, dk, positions, table, ctx.pairs, not ctx.inverse, None, False)
         return gq, gk, None, None, None, None, None, None
+
+
+def _tangent(x):
+    """(x, None), or a forward-mode dual's primal and tangent."""
+    if x is None:
+        return None, None
+    primal, tangent = forward_ad.unpack_dual(x)
+    return primal, tangent if tangent is None or tangent.stride(-1) == 1 else tangent.contiguous()
+
+
+def _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr):
+    """New rotated q and k, with what autograd wants of them: the map is
+    linear, so that a tangent goes through it as the value does."""
+    if forward_ad._current_level >= 0:
+        (q, tq), (k, tk) = _tangent(q), _tangent(k)
+        if tq is not None or tk is not None:
+            values = _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr)
+            tangents = _rotated(tq, tk, positions, table, pairs, inverse, None, pdl_attr)
+            return tuple(x if t is None else forward_ad.make_dual(x, t) for x, t in zip(values, tangents))
+    if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
+        if table.requires_grad:
+            raise ValueError("the table has no gradient")
+        return _Rotary.apply(q, k, positions, table, pairs, inverse, status, pdl_attr)
+    return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
+                        q is not None or None, k is not None or None, status, pdl_attr)
 
 
 def rotary(q, k, positions, table, *, sections: Optional[Sequence[int]] = None, interleaved: bool = False,
@@ -197,19 +222,16 @@ def rotary(q, k, positions, table, *, sections: Optional[Sequence[int]] = None, 
     `positions` (int32 or int64) is [T], or [axes, T] with `sections`: how many
     of the rot/2 pairs follow each axis -- one axis after the other, or dealt in
     turn (``interleaved``) while an axis has pairs left.  ``inverse`` turns
-    back, which is also the gradient; the call is differentiable in q and k.
-    `out_q`, `out_k` may be q and k themselves."""
+    back, which is also the gradient; the call is differentiable in q and k,
+    backward and forward, without `out_q` and `out_k`.  These may be q and k
+    themselves."""
     if stream is not None:
         with _on(q if q is not None else k, stream):
             return rotary(q, k, positions, table, sections=sections, interleaved=interleaved, pairing=pairing,
                           inverse=inverse, out_q=out_q, out_k=out_k, status=status, pdl_attr=pdl_attr)
     pairs = _pairs(table, sections, interleaved, pairing)
-    if torch.is_grad_enabled() and ((q is not None and q.requires_grad) or (k is not None and k.requires_grad)):
-        if out_q is not None or out_k is not None:
-            raise ValueError("out_q and out_k do not go with a gradient")
-        if table.requires_grad:
-            raise ValueError("the table has no gradient")
-        return _Rotary.apply(q, k, positions, table, pairs, inverse, status, pdl_attr)
+    if out_q is None and out_k is None:
+        return _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr)
     return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
                         out_q if out_q is not None else (q is not None or None),
                         out_k if out_k is not None else (k is not None or None), status, pdl_attr)

@@ -97,10 +97,15 @@ P* data(const Tensor& t) {
   return static_cast<P*>(t.data_ptr());
 }
 
-// An argument, read or written, that wants a gradient where the call has none.
+// An argument, read or written, that wants a derivative, backward or forward,
+// where the call has none.
 void no_gradient(PyObject* o, const char* call) {
-  if (!THPVariable_Check(o) || !c10::GradMode::is_enabled()) return;
-  need(!THPVariable_Unpack(o).requires_grad(), "%s has no gradient for one of its tensors that wants one: call it under torch.no_grad()", call);
+  if (!THPVariable_Check(o)) return;
+  const Tensor& t = THPVariable_Unpack(o);
+  need(!(t.requires_grad() && c10::GradMode::is_enabled()),
+       "%s has no gradient for one of its tensors that wants one: call it under torch.no_grad()", call);
+  need(!t._fw_grad(0).defined(), "%s has no forward-mode derivative for one of its tensors: call it on primal ones",
+       call);
 }
 
 // A contiguous vector of `count` values.
@@ -340,7 +345,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     a.max_position = static_cast<int>(table.size(0));
     a.rot = static_cast<int>(table.size(1));
     a.cos_sin = data<float>(table);
-    for (int i : {7, 14, 15}) no_gradient(arg[i], "rotary");
+    for (int i : {0, 1, 7, 14, 15}) no_gradient(arg[i], "rotary");
     const int64_t axes = whole(arg[8], "axes");
     need(PyBytes_Check(arg[9]) && PyBytes_GET_SIZE(arg[9]) == static_cast<Py_ssize_t>(sizeof(a.axis_of)),
          "words must be the packed axes");
@@ -365,7 +370,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     if (given(arg[5])) {
       need(q != nullptr && k != nullptr, "the cache write takes q, k and v");
       const Tensor& v = tensor(arg[2], "v");
-      for (int i : {0, 1, 2, 5, 6, 12, 13}) no_gradient(arg[i], "rotary_append");
+      for (int i : {2, 5, 6, 12, 13}) no_gradient(arg[i], "rotary_append");
       need(kind != DG_TYPE_FP32, "the cache write takes bf16 or fp16");
       need(heads_of(v, "v", x, a.v_stride) == a.kv_heads,
            "k and v must have one shape");

@@ -2,6 +2,7 @@
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fwd
 
 import decode_opt_b200 as dg
 
@@ -21,6 +22,59 @@ def _attention_inputs():
     k, v = (torch.randn(4, 8, 2, 128, generator=g, device="cuda").bfloat16() for _ in range(2))
     table = torch.arange(4, dtype=torch.int32, device="cuda").view(2, 2)
     return q, k, v, table, torch.tensor([5, 16], dtype=torch.int32, device="cuda")
+
+
+def test_rotary_forward_mode():
+    """The map is linear: its derivative along a tangent is itself."""
+    q, k, pos, table = _rotary_inputs()
+    tq, tk = torch.randn_like(q), torch.randn_like(k)
+    for pairing in ("half", "adjacent"):
+        for inverse in (False, True):
+            kw = dict(pairing=pairing, inverse=inverse)
+            want, want_t = dg.rotary(q, k, pos, table, **kw), dg.rotary(tq, tk, pos, table, **kw)
+            with fwd.dual_level():
+                got = dg.rotary(fwd.make_dual(q, tq), fwd.make_dual(k, tk), pos, table, **kw)
+                for x, y, t in zip(got, want, want_t):
+                    x = fwd.unpack_dual(x)
+                    assert torch.equal(x.primal, y) and torch.equal(x.tangent, t)
+                # One of the two, alone and beside the other; a broadcast tangent.
+                one = fwd.make_dual(q, torch.ones((), device="cuda").expand_as(q))
+                ones = dg.rotary(torch.ones_like(q), None, pos, table, **kw)[0]
+                got = dg.rotary(one, k, pos, table, **kw)
+                assert torch.equal(fwd.unpack_dual(got[0]).tangent, ones)
+                assert fwd.unpack_dual(got[1]).tangent is None and torch.equal(got[1], want[1])
+                got = dg.rotary(one, None, pos, table, **kw)
+                assert torch.equal(fwd.unpack_dual(got[0]).tangent, ones) and got[1] is None
+                with pytest.raises(ValueError):
+                    dg.rotary(one, None, pos, table, out_q=torch.empty_like(q), **kw)
+
+
+def test_forward_over_reverse():
+    """A dual that also wants a gradient: both derivatives."""
+    q, k, pos, table = _rotary_inputs()
+    t = torch.randn_like(q)
+    leaf = q.clone().requires_grad_()
+    with fwd.dual_level():
+        y = dg.rotary(fwd.make_dual(leaf, t), None, pos, table)[0]
+        assert torch.equal(fwd.unpack_dual(y).tangent, dg.rotary(t, None, pos, table)[0])
+        (g,) = torch.autograd.grad(y.sum(), leaf)
+        g = fwd.unpack_dual(g).primal
+    assert torch.equal(g, dg.rotary(torch.ones_like(q), None, pos, table, inverse=True)[0])
+
+
+def test_forward_mode_is_refused_where_there_is_no_derivative():
+    q, kc, vc, table, lens = _attention_inputs()
+    x, k, pos, rope = _rotary_inputs(torch.bfloat16)
+    cache = torch.zeros(2, 4, 2, 32, device="cuda", dtype=torch.bfloat16)
+    with fwd.dual_level():
+        with pytest.raises(ValueError):
+            dg.paged_attention(fwd.make_dual(q, torch.ones_like(q)), kc, vc, table, lens)
+        with pytest.raises(ValueError):
+            dg.paged_attention(q, kc, fwd.make_dual(vc, torch.ones_like(vc)), table, lens)
+        with pytest.raises(ValueError):
+            dg.rotary_append(x, k, fwd.make_dual(k, torch.ones_like(k)), pos, torch.arange(5, device="cuda"), cache,
+                             cache.clone(), rope)
+        dg.paged_attention(q, kc, vc, table, lens)
 
 
 def test_tensors_that_want_a_gradient_and_get_none_are_refused():
