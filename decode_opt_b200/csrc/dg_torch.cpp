@@ -108,6 +108,14 @@ void no_gradient(PyObject* o, const char* call) {
        call);
 }
 
+// A tensor that a launch has written into: what autograd saved of it is out of
+// date.  (Inference tensors have no versions.)
+void written(PyObject* o) {
+  if (!THPVariable_Check(o)) return;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A contiguous vector of `count` values.
 void vector_of(const Tensor& t, const char* name, int64_t count, c10::Device device, at::ScalarType type) {
   need(t.scalar_type() == type && t.dim() == 1 && t.size(0) == count && t.is_contiguous() && t.device() == device,
@@ -299,7 +307,11 @@ PyObject* build_block_tables(PyObject*, PyObject* const* arg, Py_ssize_t count) 
     a.requests = data<int>(*out[4]);
     a.cursor_out = data<int>(*out[5]);
     check(call_tables(&a, stream_of(device), truth(arg[9])), "dg_build_block_tables");
-    if (given(arg[7])) Py_RETURN_NONE;
+    written(arg[3]);
+    if (given(arg[7])) {
+      for (int i = 0; i < 6; ++i) written(PyTuple_GET_ITEM(arg[7], i));
+      Py_RETURN_NONE;
+    }
     PyObject* result = PyTuple_New(6);
     for (int i = 0; i < 6; ++i) PyTuple_SET_ITEM(result, i, THPVariable_Wrap(made[i]));
     return result;
@@ -412,6 +424,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
       (i == 0 ? a.q_out : a.k_out) = out->data_ptr();
     }
     check(call_rotary(&a, stream_of(device), truth(arg[17])), "dg_rotary");
+    for (int i : {5, 6, 14, 15}) written(arg[i]);
     PyObject* both = PyTuple_New(2);
     for (int i = 0; i < 2; ++i) {
       if (made[i].defined())
@@ -567,6 +580,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* arg, Py_ssize_t count) {
       a.lse = data<float>(lse);
     }
     check(call_attention(&a, stream, truth(arg[16])), "dg_paged_attention");
+    for (int i : {10, 12, 13}) written(arg[i]);
     PyObject* out = made.defined() ? THPVariable_Wrap(made) : Py_NewRef(arg[10]);
     if (!lse.defined()) return out;
     PyObject* both = PyTuple_New(2);

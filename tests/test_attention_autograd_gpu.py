@@ -109,3 +109,38 @@ def test_tensors_that_want_a_gradient_and_get_none_are_refused():
                      ((x, k, pos, rope), dict(out_q=wants(x))), ((x, k, pos, rope), dict(out_k=wants(k)))):
         with pytest.raises(ValueError):
             dg.rotary(*args, **kw)
+
+
+def test_written_tensors_have_a_new_version():
+    q, kc, vc, table, lens = _attention_inputs()
+    x, k, pos, rope = _rotary_inputs(torch.bfloat16)
+    slots = torch.arange(5, device="cuda")
+
+    def bumped(call, *tensors):
+        before = [t._version for t in tensors]
+        call()
+        return [t._version > b for t, b in zip(tensors, before)]
+    caches = [torch.zeros(2, 4, 2, 32, device="cuda", dtype=torch.bfloat16) for _ in range(2)]
+    assert all(bumped(lambda: dg.rotary_append(x, k, k, pos, slots, *caches, rope, out_q=x), x, *caches))
+    assert all(bumped(lambda: dg.rotary(x, k, pos, rope, out_q=x, out_k=k), x, k))
+    out, bits, s = q.clone(), torch.empty(2, 512, dtype=torch.uint8, device="cuda"), torch.empty(2, 4, device="cuda")
+    assert all(bumped(lambda: dg.paged_attention(q, kc, vc, table, lens, out=out, q_out=bits, q_scales=s), out, bits, s))
+    new, free = torch.ones_like(lens), torch.arange(4, 8, dtype=torch.int32, device="cuda")
+    wide = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    step = dg.build_block_tables(lens, new, free, wide, 8, 2)
+    parts = (step.seq_lens, step.query_start, step.slots, step.positions, step.requests, step.cursor)
+    assert all(bumped(lambda: dg.build_block_tables(lens, new, free, wide, 8, 2, out=step), wide, *parts))
+    # Inputs keep theirs.
+    assert not any(bumped(lambda: dg.paged_attention(q, kc, vc, table, lens), q, kc, vc, table, lens))
+    # What it is for: autograd notices that what it saved was overwritten.
+    w = torch.ones_like(q, requires_grad=True)
+    saved = q.clone()
+    loss = (w * saved).sum()
+    dg.paged_attention(q, kc, vc, table, lens, out=saved)
+    with pytest.raises(RuntimeError):
+        loss.backward()
+    # Inference tensors have no versions, and are served as before.
+    with torch.inference_mode():
+        there = torch.empty_like(q)
+    dg.paged_attention(q, kc, vc, table, lens, out=there)
+    assert torch.equal(there, out)
