@@ -18,8 +18,9 @@ pages, slots, positions) is checked there: the access is left out and `status`,
 an optional zeroed int32 tensor, receives a code (:func:`status_string`).
 Nothing synchronises; every call can be captured in a CUDA graph.  Only
 :func:`rotary` has a gradient, in q and k: a tensor that wants one elsewhere
-raises ValueError.  `stream` (default: the current one) takes a torch stream or
-a cudaStream_t handle; outputs made here are allocated on it.
+raises ValueError.  torch.jit.trace, which would keep the results as constants,
+is refused.  `stream` (default: the current one) takes a torch stream or a
+cudaStream_t handle; outputs made here are allocated on it.
 """
 
 from __future__ import annotations
@@ -60,6 +61,11 @@ def _load():
 
 
 _host = _load()
+
+
+def _untraced(name):
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError(f"torch.jit.trace cannot record {name}: its results would be constants of the trace")
 
 
 @contextlib.contextmanager
@@ -106,6 +112,7 @@ def build_block_tables(context_lens, new_lens, free_pages, block_table, page_siz
         with _on(context_lens, stream):
             return build_block_tables(context_lens, new_lens, free_pages, block_table, page_size, num_tokens,
                                       cursor=cursor, out=out, status=status, pdl_attr=pdl_attr)
+    _untraced("build_block_tables")
     if out is None:
         return StepTables(*_host.build_block_tables(context_lens, new_lens, free_pages, block_table, page_size,
                                                     num_tokens, cursor, None, status, pdl_attr))
@@ -207,6 +214,7 @@ def _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr):
         if table.requires_grad:
             raise ValueError("the table has no gradient")
         return _Rotary.apply(q, k, positions, table, pairs, inverse, status, pdl_attr)
+    _untraced("rotary")
     return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
                         q is not None or None, k is not None or None, status, pdl_attr)
 
@@ -232,6 +240,7 @@ def rotary(q, k, positions, table, *, sections: Optional[Sequence[int]] = None, 
     pairs = _pairs(table, sections, interleaved, pairing)
     if out_q is None and out_k is None:
         return _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr)
+    _untraced("rotary")
     return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
                         out_q if out_q is not None else (q is not None or None),
                         out_k if out_k is not None else (k is not None or None), status, pdl_attr)
@@ -255,6 +264,7 @@ def rotary_append(q, k, v, positions, slots, k_cache, v_cache, table, *, section
                                  out_q=out_q, status=status, pdl_attr=pdl_attr)
     if k_cache is None:
         raise ValueError("rotary_append takes the caches")
+    _untraced("rotary_append")
     return _host.rotary(q, k, v, positions, slots, k_cache, v_cache, table,
                         *_pairs(table, sections, interleaved, pairing), False, k_scale, v_scale,
                         True if out_q is None else out_q, None, status, pdl_attr)[0]
@@ -300,5 +310,6 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: Option
                                    softcap=softcap, k_scale=k_scale, v_scale=v_scale, out=out, return_lse=return_lse,
                                    q_out=q_out, q_scales=q_scales, workspace=workspace, status=status,
                                    pdl_attr=pdl_attr)
+    _untraced("paged_attention")
     return _host.paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale, window, softcap, k_scale, v_scale,
                                  out, return_lse, q_out, q_scales, workspace, status, pdl_attr)

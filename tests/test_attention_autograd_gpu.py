@@ -144,3 +144,19 @@ def test_written_tensors_have_a_new_version():
         there = torch.empty_like(q)
     dg.paged_attention(q, kc, vc, table, lens, out=there)
     assert torch.equal(there, out)
+
+
+def test_tracing_is_refused():
+    """A trace would keep the results of this one call as constants."""
+    q, kc, vc, table, lens = _attention_inputs()
+    x, k, pos, rope = _rotary_inputs(torch.bfloat16)
+    slots = torch.arange(5, device="cuda")
+    cache = torch.zeros(2, 4, 2, 32, device="cuda", dtype=torch.bfloat16)
+    free = torch.arange(4, 8, dtype=torch.int32, device="cuda")
+    for f, given in ((lambda q: dg.paged_attention(q, kc, vc, table, lens), q),
+                     (lambda q: dg.rotary(q, k, pos, rope)[0], x),
+                     (lambda q: dg.rotary_append(q, k, k, pos, slots, cache, cache.clone(), rope), x),
+                     (lambda n: dg.build_block_tables(lens, n, free, table.clone(), 8, 2).slots, torch.ones_like(lens))):
+        f(given)
+        with pytest.raises(RuntimeError, match="trace"):
+            torch.jit.trace(f, (given,), check_trace=False)
