@@ -179,14 +179,19 @@ class _Rotary(torch.autograd.Function):
     def forward(ctx, q, k, positions, table, pairs, inverse, status, pdl_attr):
         ctx.save_for_backward(positions, table)
         ctx.pairs, ctx.inverse = pairs, inverse
-        return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
-                            q is not None or None, k is not None or None, status, pdl_attr)
+        ctx.set_materialize_grads(False)
+        out = _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
+                           q is not None or None, k is not None or None, status, pdl_attr)
+        ctx.mark_non_differentiable(*(y for y, wanted in zip(out, ctx.needs_input_grad)
+                                      if y is not None and not wanted))
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dq, dk):
         positions, table = ctx.saved_tensors
-        dq, dk = (g if g is None or g.stride(-1) == 1 else g.contiguous() for g in (dq, dk))
+        dq, dk = (None if g is None or not wanted else g if g.stride(-1) == 1 else g.contiguous()
+                  for g, wanted in zip((dq, dk), ctx.needs_input_grad))
         gq = gk = None
         if dq is not None or dk is not None:
             gq, gk = _rotated(dq, dk, positions, table, ctx.pairs, not ctx.inverse, None, False)

@@ -5,6 +5,7 @@ import torch
 import torch.autograd.forward_ad as fwd
 
 import decode_opt_b200 as dg
+import decode_opt_b200.attention as attention
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +161,40 @@ def test_tracing_is_refused():
         f(given)
         with pytest.raises(RuntimeError, match="trace"):
             torch.jit.trace(f, (given,), check_trace=False)
+
+
+class _Spy:
+    """The extension module, with rotary's calls noted."""
+
+    def __init__(self, real, calls):
+        self.real, self.calls = real, calls
+
+    def __getattr__(self, name):
+        return getattr(self.real, name)
+
+    def rotary(self, *args):
+        self.calls.append(args)
+        return self.real.rotary(*args)
+
+
+def test_backward_turns_back_what_is_wanted_only(monkeypatch):
+    q, k, pos, table = _rotary_inputs()
+    calls = []
+    monkeypatch.setattr(attention, "_host", _Spy(attention._host, calls))
+    for wq, wk in ((True, False), (False, True), (True, True)):
+        a, b = q.clone().requires_grad_(wq), k.clone().requires_grad_(wk)
+        y, z = dg.rotary(a, b, pos, table)
+        assert (y.requires_grad, z.requires_grad) == (wq, wk)
+        del calls[:]
+        (sum(t.sum() for t in (y, z) if t.requires_grad)).backward()
+        assert [(c[0] is not None, c[1] is not None) for c in calls] == [(wq, wk)]
+        for t, g in ((a, q), (b, k)):
+            if t.requires_grad:
+                ones = torch.ones_like(g)
+                assert torch.equal(t.grad, dg.rotary(ones, None, pos, table, inverse=True)[0])
+    # Both could have one, and only one result is used.
+    a, b = q.clone().requires_grad_(), k.clone().requires_grad_()
+    y, _ = dg.rotary(a, b, pos, table)
+    del calls[:]
+    ga, gb = torch.autograd.grad(y.sum(), (a, b), allow_unused=True)
+    assert len(calls) == 1 and calls[0][1] is None and gb is None and ga is not None
