@@ -14,6 +14,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -114,6 +115,14 @@ void written(PyObject* o) {
   if (!THPVariable_Check(o)) return;
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+// An output with a place for each of its values, and none of them in another
+// place of `in` (it may be `in` itself).
+void apart(const Tensor& out, const Tensor* in, const char* name) {
+  need(at::has_internal_overlap(out) != at::MemOverlap::Yes, "%s has several values in one place", name);
+  need(in == nullptr || at::get_overlap_status(out, *in) != at::MemOverlapStatus::Partial,
+       "%s partly overlaps its input", name);
 }
 
 // A contiguous vector of `count` values.
@@ -390,6 +399,11 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
       const Tensor& vc = tensor(arg[6], "v_cache");
       const Cache c = cache_of(kc, vc, a.kv_heads, x, a.k_cache_stride,
                                a.v_cache_stride);
+      apart(kc, nullptr, "k_cache");
+      apart(vc, nullptr, "v_cache");
+      const auto overlap = at::get_overlap_status(kc, vc);
+      need(overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial,
+           "k_cache and v_cache must not overlap");
       const Tensor& slots = tensor(arg[4], "slots");
       vector_of(slots, "slots", tokens, device, at::kLong);
       a.v = v.data_ptr();
@@ -416,6 +430,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
         made[i] = at::empty({tokens, heads, dim}, at::TensorOptions().device(device).dtype(x.scalar_type()));
       } else {
         out = &tensor(o, i == 0 ? "out_q" : "out_k");
+        apart(*out, in, i == 0 ? "out_q" : "out_k");
         result[i] = o;
       }
       auto& stride = i == 0 ? a.q_out_stride : a.k_out_stride;
@@ -539,6 +554,7 @@ PyObject* paged_attention(PyObject*, PyObject* const* arg, Py_ssize_t count) {
       const Tensor& out = tensor(arg[10], "out");
       need(heads_of(out, "out", q, a.out_stride) == heads,
            "out must have q's shape");
+      apart(out, nullptr, "out");
       a.out = out.data_ptr();
     }
     if (given(arg[12]) || given(arg[13])) {

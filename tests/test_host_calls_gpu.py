@@ -80,3 +80,36 @@ def test_a_free_list_inside_the_block_table_is_refused():
     assert table[:, 0].tolist() == [6, 7, 8] and got.cursor.tolist() == [3]
     got = dg.build_block_tables(lens, new, wide[2, 7:], table, 4, 3)
     assert table[:, 0].tolist() == [27, 28, 29] and got.slots.tolist() == [108, 112, 116]
+
+
+def test_outputs_that_overlap_are_refused():
+    """An output with several values in one place, or one that is moved a
+    little against its own input, would be written and read in no order."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(4, 2, 64, generator=g, device="cuda").bfloat16()
+    pos, rope, slots = torch.arange(4, device="cuda"), dg.rope_table(8, 64), torch.arange(4, device="cuda")
+    flat = torch.zeros(5 * 128, dtype=torch.bfloat16, device="cuda")
+    a, b = flat[:512].view(4, 2, 64), flat[128:].view(4, 2, 64)
+    one = torch.zeros(1, 2, 64, dtype=torch.bfloat16, device="cuda")
+    cache = torch.zeros(2, 4, 2, 64, dtype=torch.bfloat16, device="cuda")
+    flat_cache = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device="cuda").expand(2, 4, 2, 64)
+    for kw in (dict(out_q=one.expand(4, 2, 64)), dict(out_k=one.expand(4, 2, 64))):
+        with pytest.raises(ValueError):
+            dg.rotary(q, q, pos, rope, **kw)
+    for x, y in ((a, b), (b, a)):
+        with pytest.raises(ValueError):
+            dg.rotary(x, None, pos, rope, out_q=y)
+        with pytest.raises(ValueError):
+            dg.rotary(None, x, pos, rope, out_k=y)
+    for caches in ((flat_cache, cache), (cache, flat_cache)):
+        with pytest.raises(ValueError):
+            dg.rotary_append(q, q, q, pos, slots, *caches, rope)
+    with pytest.raises(ValueError):
+        dg.rotary_append(q, q, q, pos, slots, cache, cache, rope)
+    table, lens = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), torch.ones(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        dg.paged_attention(q, cache, cache, table, lens, out=one.expand(4, 2, 64))
+    # The input itself is a fine output, and a cache that is only read may be one tensor with many names.
+    want = dg.rotary(q, None, pos, rope)[0]
+    assert torch.equal(dg.rotary(q, None, pos, rope, out_q=q)[0], want)
+    dg.paged_attention(q, flat_cache, flat_cache, table, lens)
