@@ -1213,6 +1213,10 @@ bool refused(const dg_attention_args& a) {
   if (!(a.softcap >= 0.0f) || !(a.scale == a.scale)) return true;
   if ((reinterpret_cast<uintptr_t>(a.q) & 3u) != 0 || a.q_stride[0] % 2 != 0 || a.q_stride[1] % 2 != 0) return true;
   if (((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 15u) != 0) return true;
+  if ((reinterpret_cast<uintptr_t>(a.out) & 1u) != 0) return true;
+  const void* words[] = {a.block_table, a.seq_lens, a.k_scale, a.v_scale, a.lse, a.q_scales, a.status};
+  for (const void* p : words)
+    if ((reinterpret_cast<uintptr_t>(p) & 3u) != 0) return true;
   for (int i = 0; i < 3; ++i)
     if (a.k_cache_stride[i] % (e4m3 ? 16 : 8) != 0 || a.v_cache_stride[i] % (e4m3 ? 16 : 8) != 0) return true;
   if ((a.q_out != nullptr) != (a.q_scales != nullptr)) return true;

@@ -285,6 +285,10 @@ extern "C" int dg_build_block_tables(const dg_block_tables* args, void* stream, 
       a.query_start == nullptr || a.cursor_out == nullptr || (a.free_count > 0 && a.free_pages == nullptr) ||
       (a.num_tokens > 0 && (a.slots == nullptr || a.positions == nullptr || a.requests == nullptr)))
     return cudaErrorInvalidValue;
+  const void* ints[] = {a.context_lens, a.new_lens, a.free_pages, a.cursor_in, a.block_table, a.seq_lens,
+                        a.query_start, a.positions, a.requests, a.cursor_out, a.status};
+  for (const void* p : ints)
+    if ((reinterpret_cast<uintptr_t>(p) & 3u) != 0) return cudaErrorInvalidValue;
   if ((reinterpret_cast<uintptr_t>(a.slots) & 7u) != 0) return cudaErrorInvalidValue;
   // Other CTAs read these while CTA 0 writes.
   if (a.seq_lens == a.context_lens || a.seq_lens == a.new_lens || a.cursor_out == a.cursor_in)

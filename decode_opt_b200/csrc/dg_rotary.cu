@@ -396,6 +396,14 @@ bool refused(const dg_rotary_args& a) {
   if (a.positions == nullptr || a.cos_sin == nullptr || a.position_stride < 0) return true;
   if ((a.heads > 0) != (a.q != nullptr) || (a.q != nullptr) != (a.q_out != nullptr)) return true;
   if ((a.kv_heads > 0) != (a.k != nullptr)) return true;
+  const uintptr_t value = a.type == DG_TYPE_FP32 ? 3 : 1, place = a.position_64 != 0 ? 7 : 3;
+  const void* values[] = {a.q, a.k, a.v, a.q_out, a.k_out};
+  for (const void* p : values)
+    if ((reinterpret_cast<uintptr_t>(p) & value) != 0) return true;
+  const void* words[] = {a.cos_sin, a.k_scale, a.v_scale, a.status};
+  for (const void* p : words)
+    if ((reinterpret_cast<uintptr_t>(p) & 3u) != 0) return true;
+  if ((reinterpret_cast<uintptr_t>(a.positions) & place) != 0) return true;
   const bool cached = a.k_cache != nullptr;
   if (cached != (a.v_cache != nullptr) || cached != (a.v != nullptr)) return true;
   if (a.k != nullptr && a.k_out == nullptr && !cached) return true;
@@ -403,6 +411,10 @@ bool refused(const dg_rotary_args& a) {
   if (cached) {
     if (a.slots == nullptr || a.page_size < 1 || a.num_pages < 1) return true;
     if (a.type == DG_TYPE_FP32 || (a.cache_type != a.type && a.cache_type != DG_TYPE_E4M3)) return true;
+    if ((reinterpret_cast<uintptr_t>(a.slots) & 7u) != 0) return true;
+    if (a.cache_type != DG_TYPE_E4M3 &&
+        ((reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache)) & 1u) != 0)
+      return true;
     if (a.cache_type != DG_TYPE_E4M3 && (a.k_scale != nullptr || a.v_scale != nullptr)) return true;
   }
   return false;

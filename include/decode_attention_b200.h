@@ -19,7 +19,8 @@
  * programmatic stream serialization; every kernel waits for the kernels before
  * it on the stream before it reads or writes global memory.
  *
- * Strides are in elements.  The last dimension of every tensor is contiguous.
+ * Strides are in elements.  The last dimension of every tensor is contiguous,
+ * its address a multiple of its elements' size (refused otherwise).
  */
 #ifndef DECODE_ATTENTION_B200_H_
 #define DECODE_ATTENTION_B200_H_
