@@ -65,7 +65,8 @@ def needs_build(target: str = LIB_PATH, extra=()) -> bool:
 
 
 def build(verbose: bool = False, ptxas_verbose: bool = False, force: bool = False) -> str:
-    lib = build_library(verbose, ptxas_verbose, force)
+    lib = build_cuda(verbose, ptxas_verbose, force)
+    build_host(verbose, force)
     build_drop_in_check(verbose, force)
     build_cublaslt_bench(verbose, force)
     return lib
@@ -77,6 +78,8 @@ def build_host(verbose: bool = False, force: bool = False) -> str:
     if not force and os.path.exists(HOST_LIB) and \
             os.path.getmtime(HOST_LIB) > max(os.path.getmtime(HOST_SRC), os.path.getmtime(header)):
         return HOST_LIB
+    if os.path.exists(HOST_LIB):
+        os.remove(HOST_LIB)          # of other sources: it would pass structs of another layout
     import sysconfig
 
     import torch
@@ -92,6 +95,17 @@ def build_host(verbose: bool = False, force: bool = False) -> str:
     subprocess.run(cmd, check=True)
     os.replace(HOST_LIB + ".tmp", HOST_LIB)
     return HOST_LIB
+
+
+def build_library(verbose: bool = False, ptxas_verbose: bool = False, force: bool = False) -> str:
+    """The C library, which needs no torch; then the extension module, without
+    which attention.py says so when it is first used."""
+    lib = build_cuda(verbose, ptxas_verbose, force)
+    try:
+        build_host(verbose, force)
+    except (ImportError, OSError, subprocess.CalledProcessError) as e:
+        print(f"{HOST_LIB} was not built: {e}", file=sys.stderr)
+    return lib
 
 
 def cuda_lib_dir() -> str:
@@ -126,10 +140,9 @@ def build_drop_in_check(verbose: bool = False, force: bool = False) -> str:
     return DROP_IN_BIN
 
 
-def build_library(verbose: bool = False, ptxas_verbose: bool = False, force: bool = False) -> str:
-    """The library and the extension module that calls it from torch."""
-    build_host(verbose, force)
-    if not force and not needs_build():
+def build_cuda(verbose: bool = False, ptxas_verbose: bool = False, force: bool = False) -> str:
+    """The C library alone."""
+    if not force and not needs_build(LIB_PATH):
         return LIB_PATH
     cmd = [nvcc(), "-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS,
            "-Xcompiler", "-fPIC", "-shared", "-cudart", "static", "--threads", "0",

@@ -1,0 +1,55 @@
+"""CPU tests of the build recipe: what is built from what, and what a failure
+leaves.  No compiler is run."""
+
+import os
+import subprocess
+
+import pytest
+
+from decode_opt_b200 import build as dg_build
+
+
+class Compilers:
+    """Stands in for subprocess.run: notes the outputs asked for, makes them
+    (empty files), and fails for those named."""
+
+    def __init__(self, failing=()):
+        self.made, self.failing = [], failing
+
+    def __call__(self, cmd, check=False, **kw):
+        out = cmd[cmd.index("-o") + 1]
+        name = os.path.basename(out).removesuffix(".tmp")
+        self.made.append(name)
+        if name in self.failing:
+            raise subprocess.CalledProcessError(1, cmd)
+        open(out, "wb").close()
+        return subprocess.CompletedProcess(cmd, 0)
+
+
+@pytest.fixture
+def place(tmp_path, monkeypatch):
+    """The build's outputs in a folder of their own."""
+    for name in ("LIB_PATH", "HOST_LIB", "DROP_IN_BIN", "CUBLASLT_BIN"):
+        monkeypatch.setattr(dg_build, name, str(tmp_path / os.path.basename(getattr(dg_build, name))))
+    return tmp_path
+
+
+@pytest.mark.parametrize("force", [False, True])
+def test_the_library_needs_no_torch(place, monkeypatch, force):
+    """A host compiler that refuses torch's headers, or no torch at all: the C
+    library is built all the same, and no extension module of before is left
+    beside it."""
+    run = Compilers(failing=("_host.so",))
+    monkeypatch.setattr(subprocess, "run", run)
+    (place / "_host.so").write_bytes(b"of another build")
+    os.utime(place / "_host.so", (1, 1))
+    assert dg_build.build_library(force=force) == dg_build.LIB_PATH
+    assert run.made[0] == "libdecode_gemm_b200.so" and os.path.exists(dg_build.LIB_PATH)
+    assert not os.path.exists(dg_build.HOST_LIB)
+    # The whole build says so.
+    with pytest.raises(subprocess.CalledProcessError):
+        dg_build.build(force=force)
+    monkeypatch.setitem(__import__("sys").modules, "torch", None)
+    assert dg_build.build_library(force=True) == dg_build.LIB_PATH
+    with pytest.raises(ImportError):
+        dg_build.build(force=True)
