@@ -53,7 +53,9 @@ def nvcc() -> str:
 
 
 def _sources():
-    return [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC))] + [
+    """What the nvcc-built programs are made of (the extension module's source
+    is host code for torch's headers, and none of theirs)."""
+    return [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f != os.path.basename(HOST_SRC)] + [
         os.path.join(INCLUDE, f) for f in sorted(os.listdir(INCLUDE))]
 
 

@@ -53,3 +53,22 @@ def test_the_library_needs_no_torch(place, monkeypatch, force):
     assert dg_build.build_library(force=True) == dg_build.LIB_PATH
     with pytest.raises(ImportError):
         dg_build.build(force=True)
+
+
+def test_host_code_does_not_recompile_the_kernels(place, monkeypatch):
+    run = Compilers()
+    monkeypatch.setattr(subprocess, "run", run)
+    dg_build.build()
+    assert sorted(run.made) == ["_host.so", "dg_cublaslt_fp8", "dg_drop_in_check", "libdecode_gemm_b200.so"]
+    real = os.path.getmtime
+    ahead = set()
+    monkeypatch.setattr(os.path, "getmtime", lambda p: real(p) + 10 ** 6 * (str(p) in ahead))
+    ahead.add(dg_build.HOST_SRC)
+    assert not dg_build.needs_build(dg_build.LIB_PATH)
+    for source in dg_build.SOURCES + ("sm100.cuh", "warp_mma.cuh"):
+        ahead.clear()
+        ahead.add(os.path.join(dg_build.CSRC, source))
+        assert dg_build.needs_build(dg_build.LIB_PATH), source
+    ahead.clear()
+    ahead.add(os.path.join(dg_build.INCLUDE, "decode_attention_b200.h"))
+    assert dg_build.needs_build(dg_build.LIB_PATH)
