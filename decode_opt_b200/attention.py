@@ -37,7 +37,7 @@ from typing import Optional, Sequence, Tuple
 import torch
 from torch.autograd import forward_ad
 
-from . import _lib
+from . import _lib, build
 
 __all__ = ["StepTables", "build_block_tables", "rope_table", "rotary", "rotary_append", "paged_attention",
            "attention_workspace"]
@@ -54,6 +54,8 @@ def _load():
     spec = importlib.util.spec_from_file_location("decode_opt_b200._host", HOST_PATH)
     host = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(host)
+    if host.built_for != build.host_built_for():
+        raise RuntimeError(f"{HOST_PATH} is the {host.built_for}: build it again with `python -m decode_opt_b200.build`")
     lib = _lib.lib()
     host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
         "dg_build_block_tables", "dg_rotary", "dg_paged_attention", "dg_attention_workspace_bytes")))

@@ -74,11 +74,26 @@ def build(verbose: bool = False, ptxas_verbose: bool = False, force: bool = Fals
     return lib
 
 
+def host_built_for() -> str:
+    """What the extension module is compiled against, as it says itself
+    (``_host.built_for``)."""
+    import torch
+    python = f"{sys.version_info[0]}.{sys.version_info[1]}"
+    return f"decode_opt_b200 host extension for torch {torch.__version__}, Python {python}"
+
+
+def host_needs_build() -> bool:
+    header = os.path.join(INCLUDE, "decode_attention_b200.h")
+    if not os.path.exists(HOST_LIB) or \
+            os.path.getmtime(HOST_LIB) <= max(os.path.getmtime(HOST_SRC), os.path.getmtime(header)):
+        return True
+    with open(HOST_LIB, "rb") as f:
+        return host_built_for().encode() + b"\0" not in f.read()
+
+
 def build_host(verbose: bool = False, force: bool = False) -> str:
     """The extension module of the attention operators' calls."""
-    header = os.path.join(INCLUDE, "decode_attention_b200.h")
-    if not force and os.path.exists(HOST_LIB) and \
-            os.path.getmtime(HOST_LIB) > max(os.path.getmtime(HOST_SRC), os.path.getmtime(header)):
+    if not force and not host_needs_build():
         return HOST_LIB
     if os.path.exists(HOST_LIB):
         os.remove(HOST_LIB)          # of other sources: it would pass structs of another layout
@@ -89,7 +104,8 @@ def build_host(verbose: bool = False, force: bool = False) -> str:
     flags = [f"-I{os.path.join(root, 'include')}", f"-I{os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include')}",
              f"-I{sysconfig.get_paths()['include']}", f"-I{os.path.join(cuda_lib_dir(), '..', 'include')}", f"-I{INCLUDE}"]
     cmd = [os.environ.get("CXX", "g++"), "-std=c++17", "-O2", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *flags, HOST_SRC, "-o",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DDG_BUILT_FOR="{host_built_for()}"', *flags, HOST_SRC, "-o",
            HOST_LIB + ".tmp", "-L", os.path.join(root, "lib"), "-L", cuda_lib_dir(), "-lc10", "-lc10_cuda", "-ltorch",
            "-ltorch_cpu", "-ltorch_python", "-lcudart"]
     if verbose:

@@ -638,4 +638,10 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, null
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host(void) { return PyModule_Create(&module); }
+// Compiled against the torch and Python that the build names here: the module
+// is of no use to others.
+PyMODINIT_FUNC PyInit__host(void) {
+  PyObject* m = PyModule_Create(&module);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", DG_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -72,3 +72,32 @@ def test_host_code_does_not_recompile_the_kernels(place, monkeypatch):
     ahead.clear()
     ahead.add(os.path.join(dg_build.INCLUDE, "decode_attention_b200.h"))
     assert dg_build.needs_build(dg_build.LIB_PATH)
+
+
+def test_another_torch_means_another_extension(place, monkeypatch):
+    import torch
+    host = place / "_host.so"
+    assert dg_build.host_needs_build()
+    host.write_bytes(b"code" + dg_build.host_built_for().encode() + b"\0more code")
+    assert not dg_build.host_needs_build()
+    monkeypatch.setattr(torch, "__version__", torch.__version__ + ".1")
+    assert dg_build.host_needs_build()
+    run = Compilers()
+    monkeypatch.setattr(subprocess, "run", run)
+    dg_build.build_host()
+    assert run.made == ["_host.so"]
+
+
+def test_the_extension_says_what_it_was_built_for():
+    """(In a process of its own: it loads torch's libraries.)"""
+    import sys
+    code = ("import decode_opt_b200.attention as a, decode_opt_b200.build as b; "
+            "print(a._host.built_for == b.host_built_for(), b.host_needs_build())")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=dg_build.ROOT)
+    assert out.stdout.split() == ["True", "False"], out.stderr
+    # ... and another torch does not run it.
+    code = ("import torch; torch.__version__ = '0.0.1'\n"
+            "try: import decode_opt_b200.attention\n"
+            "except RuntimeError as e: print('build it again' in str(e))")
+    out = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, cwd=dg_build.ROOT)
+    assert out.stdout.split() == ["True"], out.stderr
