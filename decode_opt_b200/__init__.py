@@ -39,6 +39,8 @@ The operators between two products of a decode layer -- block tables
 from __future__ import annotations
 
 import ctypes
+import importlib.util
+import os
 from dataclasses import dataclass, field
 from typing import Optional
 
@@ -56,14 +58,15 @@ __all__ = [
     "LAYOUT_RAW", "LAYOUT_PACKED", "LAYOUT_PACKED_SWIZZLED", "FLAG_INJECT_TIMEOUT", "FLAG_INDEPENDENT_INPUTS",
     "FLAG_SWAP_AB",
     "ERR_INJECTED_TIMEOUT", "STATUS_OK", "m_tile_for", "flush_l2", "GRID_CLUSTER", "copy_from_host",
-    "StepTables", "build_block_tables", "rope_table", "rotary", "rotary_append", "paged_attention",
-    "attention_workspace",
 ]
 
 # The attention operators (attention.py): loaded on first use, as that module
-# imports torch and this one does not.
+# imports torch and this one does not; names of the star import where that can
+# be done.
 _ATTENTION = frozenset(("StepTables", "build_block_tables", "rope_table", "rotary", "rotary_append",
                         "paged_attention", "attention_workspace"))
+if importlib.util.find_spec("torch") is not None and os.path.exists(os.path.join(os.path.dirname(__file__), "_host.so")):
+    __all__ += sorted(_ATTENTION)
 
 
 def __getattr__(name):
@@ -72,6 +75,10 @@ def __getattr__(name):
         globals()[name] = value = getattr(attention, name)
         return value
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
+def __dir__():
+    return sorted(_ATTENTION.union(globals()))
 
 
 CUDA_SUCCESS = 0
