@@ -65,11 +65,6 @@ def _load():
 _host = _load()
 
 
-def _untraced(name):
-    if torch._C._get_tracing_state() is not None:
-        raise RuntimeError(f"torch.jit.trace cannot record {name}: its results would be constants of the trace")
-
-
 @contextlib.contextmanager
 def _on(tensor, stream):
     """With the tensor's device and `stream` current."""
@@ -114,7 +109,6 @@ def build_block_tables(context_lens, new_lens, free_pages, block_table, page_siz
         with _on(context_lens, stream):
             return build_block_tables(context_lens, new_lens, free_pages, block_table, page_size, num_tokens,
                                       cursor=cursor, out=out, status=status, pdl_attr=pdl_attr)
-    _untraced("build_block_tables")
     if out is None:
         return StepTables(*_host.build_block_tables(context_lens, new_lens, free_pages, block_table, page_size,
                                                     num_tokens, cursor, None, status, pdl_attr))
@@ -200,6 +194,13 @@ class _Rotary(torch.autograd.Function):
         return gq, gk, None, None, None, None, None, None
 
 
+def _untraced():
+    """(The other calls look for themselves; rotary's gradient is an operation
+    that a trace records.)"""
+    if torch._C._get_tracing_state() is not None:
+        raise RuntimeError("torch.jit.trace cannot record rotary: its results would be constants of the trace")
+
+
 def _tangent(x):
     """(x, None), or a forward-mode dual's primal and tangent."""
     if x is None:
@@ -221,7 +222,7 @@ def _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr):
         if table.requires_grad:
             raise ValueError("the table has no gradient")
         return _Rotary.apply(q, k, positions, table, pairs, inverse, status, pdl_attr)
-    _untraced("rotary")
+    _untraced()
     return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
                         q is not None or None, k is not None or None, status, pdl_attr)
 
@@ -247,7 +248,7 @@ def rotary(q, k, positions, table, *, sections: Optional[Sequence[int]] = None, 
     pairs = _pairs(table, sections, interleaved, pairing)
     if out_q is None and out_k is None:
         return _rotated(q, k, positions, table, pairs, inverse, status, pdl_attr)
-    _untraced("rotary")
+    _untraced()
     return _host.rotary(q, k, None, positions, None, None, None, table, *pairs, inverse, None, None,
                         out_q if out_q is not None else (q is not None or None),
                         out_k if out_k is not None else (k is not None or None), status, pdl_attr)
@@ -271,7 +272,6 @@ def rotary_append(q, k, v, positions, slots, k_cache, v_cache, table, *, section
                                  out_q=out_q, status=status, pdl_attr=pdl_attr)
     if k_cache is None:
         raise ValueError("rotary_append takes the caches")
-    _untraced("rotary_append")
     return _host.rotary(q, k, v, positions, slots, k_cache, v_cache, table,
                         *_pairs(table, sections, interleaved, pairing), False, k_scale, v_scale,
                         True if out_q is None else out_q, None, status, pdl_attr)[0]
@@ -317,6 +317,5 @@ def paged_attention(q, k_cache, v_cache, block_table, seq_lens, *, scale: Option
                                    softcap=softcap, k_scale=k_scale, v_scale=v_scale, out=out, return_lse=return_lse,
                                    q_out=q_out, q_scales=q_scales, workspace=workspace, status=status,
                                    pdl_attr=pdl_attr)
-    _untraced("paged_attention")
     return _host.paged_attention(q, k_cache, v_cache, block_table, seq_lens, scale, window, softcap, k_scale, v_scale,
                                  out, return_lse, q_out, q_scales, workspace, status, pdl_attr)

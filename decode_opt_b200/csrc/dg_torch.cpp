@@ -15,6 +15,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/MemoryOverlap.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -98,10 +99,14 @@ P* data(const Tensor& t) {
   return static_cast<P*>(t.data_ptr());
 }
 
+// An argument that may be a tensor: not None, nor a truth value (asked first,
+// as asking those whether they are tensors takes Python 0.1 us each).
+bool some_tensor(PyObject* o) { return o != Py_None && !PyBool_Check(o) && THPVariable_Check(o); }
+
 // An argument, read or written, that wants a derivative, backward or forward,
 // where the call has none.
 void no_gradient(PyObject* o, const char* call) {
-  if (!THPVariable_Check(o)) return;
+  if (!some_tensor(o)) return;
   const Tensor& t = THPVariable_Unpack(o);
   need(!(t.requires_grad() && c10::GradMode::is_enabled()),
        "%s has no gradient for one of its tensors that wants one: call it under torch.no_grad()", call);
@@ -109,10 +114,18 @@ void no_gradient(PyObject* o, const char* call) {
        call);
 }
 
+// torch.jit.trace records no calls of this module: their results would be
+// constants of the trace.
+void no_trace(const char* call) {
+  if (at::tracer::impl::is_dispatch_enabled())
+    throw std::runtime_error(std::string("torch.jit.trace cannot record ") + call +
+                             ": its results would be constants of the trace");
+}
+
 // A tensor that a launch has written into: what autograd saved of it is out of
 // date.  (Inference tensors have no versions.)
 void written(PyObject* o) {
-  if (!THPVariable_Check(o)) return;
+  if (!some_tensor(o)) return;
   const Tensor& t = THPVariable_Unpack(o);
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -242,6 +255,7 @@ PyObject* guarded(F body) {
 PyObject* build_block_tables(PyObject*, PyObject* const* arg, Py_ssize_t count) {
   COUNT(10)
   return guarded([&]() -> PyObject* {
+    no_trace("build_block_tables");
     const Tensor& context = tensor(arg[0], "context_lens");
     const Tensor& fresh = tensor(arg[1], "new_lens");
     const Tensor& free_pages = tensor(arg[2], "free_pages");
@@ -389,6 +403,7 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     a.position_64 = wide;
     a.status = status_of(arg[16], device);
     if (given(arg[5])) {
+      no_trace("rotary_append");
       need(q != nullptr && k != nullptr, "the cache write takes q, k and v");
       const Tensor& v = tensor(arg[2], "v");
       for (int i : {2, 5, 6, 12, 13}) no_gradient(arg[i], "rotary_append");
@@ -486,6 +501,7 @@ Tensor stream_workspace(c10::Device device, void* stream) {
 PyObject* paged_attention(PyObject*, PyObject* const* arg, Py_ssize_t count) {
   COUNT(17)
   return guarded([&]() -> PyObject* {
+    no_trace("paged_attention");
     const Tensor& q = tensor(arg[0], "q");
     const Tensor& kc = tensor(arg[1], "k_cache");
     const Tensor& vc = tensor(arg[2], "v_cache");
