@@ -3,17 +3,19 @@
 // dg_attention.cu -- attention of one new token per request over a paged
 // key-value cache (include/decode_attention_b200.h gives the definition).
 //
-// Bound: the live tokens' keys and values are read once per kv head, 2 * D
-// values a token, against 4 * D operations a token and query head: HBM
-// traffic by its numbers for any group of heads that is served here.  What a
-// kernel meets before that is the rate at which 8 warps an SM (their rings and
-// accumulators fill shared memory and registers) get through the instructions
-// of a tile: 16 tokens of 16-bit keys and 8 heads keep up with HBM, 32 tokens
-// of e4m3 and 16 heads do not.
-// B200: 1.05M tokens of 4 heads of 128, bf16, 8 query heads each (2.15 GB):
-// 0.33 ms, 6.7 TB/s, 105% of a copy's rate; a ragged batch of 61 requests on 8
-// heads (0.70 GB) 122 us, 5.7 TB/s; 64 requests in e4m3 under 16 query heads
-// a kv head (1.0 GB) 217 us, 4.7 TB/s; one request of 2049 tokens 9.5 us.
+// Bound: the live tokens' keys and values are read once per kv head (for up to
+// 16 query heads a kv head; more read them once per 16), 2 * D values a token,
+// against 4 * D operations a token and query head: HBM traffic by its numbers.
+// What a kernel meets before that is the rate at which 8 warps an SM (their
+// rings and accumulators fill shared memory and registers) get through the
+// instructions of a tile: 16 tokens of 16-bit keys and 8 heads keep up with
+// HBM, 32 tokens of e4m3 and 16 heads do not, nor do heads of 256 (spills).
+// B200, calls one after another (in a graph): 1.08M tokens of 4 heads of 128,
+// bf16, 8 query heads each (2.21 GB) 333 us (330), 6.6 TB/s, 104% of a copy's
+// rate; a ragged batch of 61 requests on 8 heads (0.70 GB) 124 us (123), 5.7
+// TB/s; 64 requests in e4m3 under 16 query heads a kv head (1.0 GB) 233 us
+// (221), 4.4 TB/s; 64 heads on 4 of 256 on the ragged lengths 220 us (218), 3.2
+// TB/s; one request of 2049 tokens 10.9 us (9.8).
 //
 // Split.  The work is cut into tiles of TOK tokens of one (request, kv head,
 // group of ROWS query heads) "item"; all tiles of all items stand in one
@@ -32,17 +34,25 @@
 // strides; tokens that are not live are zero-filled and masked.
 //
 // Products: mma.sync m16n8k16, the query heads as its 16 rows.  The tensor
-// pipe is a third busy at most (39% with e4m3 and 16 heads), so that the
-// roomier tcgen05 shapes (64 or 128 rows) would multiply zeros, and their
-// operands from shared memory would want e4m3 widened there first.  Scores
-// stay in registers: the accumulator
+// pipe is 16 to 19% busy with 16-bit caches, 42% with e4m3 and 16 heads an item
+// (of active cycles).  tcgen05's 64 or 128 rows would multiply zeros with
+// the heads as rows; with keys, then values, as rows and the heads as columns
+// they would be full, and e4m3 would need no widening.  16-bit caches of heads
+// up to 128 under up to 16 heads have little to gain from that (80 to 104% of a
+// copy's rate); wider heads, larger groups and e4m3 with more than 8 heads
+// would, and it is not built.
+//
+// Scores stay in registers: the accumulator
 // layout of S = Q K^T is the operand layout of P V.  P enters as two terms,
-// hi = p cut to 16 bits and lo = round(p - hi), so that its rounding (2^-8 in
-// bf16) does not show in the result: with up to 8 query heads a kv head
+// hi = p cut to 16 bits and lo = round(p - hi): 16 to 17 bits of p with bf16
+// caches, 22 with fp16 and e4m3, so that its rounding (2^-8 in bf16) does not
+// show in the result.  (Ragged batch, against the value in 64 bits rounded
+// once: 3.6 of 1000 bf16 outputs round the other way, 0.7 in 32 bits; the
+// error of either is 1.66e-3.)  With up to 8 query heads a kv head
 // (ROWS = 8) the lo terms fill the 8 rows that would be empty, at no cost;
 // with more (ROWS = 16) they are a second product.  Cut towards zero and with
 // lo kept above 0, both terms have the sign of p, so that an infinite value
-// stays infinite (0 times it would be NaN).
+// stays infinite (0 times it would be NaN) where p itself is not 0.
 //
 // e4m3 caches are widened to fp16 (exact) on the way into the product.  Both
 // products are indifferent to the order of their inner index, and the columns
@@ -127,8 +137,10 @@ struct Shape {
   static constexpr int SOLO = 8;                                 // tiles of an item that one warp does alone
   // What an item costs beyond its tiles (join, uneven warps), in tiles: CTAs
   // with 3 and with 15 items of the same units differed by 1.7 to 4.5 us an
-  // item.  Ragged batch, 8 heads an item: 129.8 us at 4, 123.7 at 8, 123.0 at
-  // 14, 122.7 at 20; 16 heads: 161.7, 149.9, 142.1, 135.4.
+  // item.  One figure for tiles of all head dimensions, whose times differ;
+  // measured with heads of 128.  Ragged batch, 8 heads an item: 129.8 us at 4,
+  // 123.7 at 8, 123.0 at 14, 122.7 at 20; 16 heads: 161.7, 149.9, 142.1, 135.4
+  // (still falling at 20, and not tried beyond).
   static constexpr int EXTRA_SOLO = 1, EXTRA = ROWS_ == 8 ? 14 : 20;
   static constexpr int MIN_RUN = 8;                              // units a CTA takes at least
   static constexpr int NT = TOK / 8;                             // score tiles of 8 tokens

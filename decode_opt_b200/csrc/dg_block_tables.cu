@@ -18,7 +18,7 @@
 // read from the table, a later one from the free list itself.
 //
 // Bound: the launch, three dependent loads and the scan for a decode step
-// (B200, in a graph: 4.4 us for 16 requests, 5.8 for 512); the searches'
+// (B200, in a graph: 4.5 us for 16 requests, 5.9 for 512); the searches'
 // instructions at the other end (4096 prompts, 1.4 million tokens, 23 MB:
 // 16 us, where the bytes alone would take 3.6).
 

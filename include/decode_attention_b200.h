@@ -137,10 +137,15 @@ int dg_rotary(const dg_rotary_args* args, void* stream, int pdl_attr);
    over the live tokens t in [max(0, len - window), len), len = seq_lens[b]
    (window 0: all of them); token t lies at offset t % page_size of page
    block_table[b, t / page_size].  A request without live tokens gives 0 and
-   lse -inf.  Memory outside the live tokens is never read, whatever it holds.
+   lse -inf; so does one whose live tokens are all left out for bad pages
+   (DG_ERR_PAGE).  Memory outside the live tokens is never read, whatever it
+   holds.  A NaN among the live tokens makes out and lse NaN, for the heads that
+   read it.
    Products of the stored values accumulate in fp32; probabilities enter the
-   second product as two terms of the cache's 16-bit type (fp16 for e4m3), so
-   that only the result is rounded; sums and maxima are fp32.
+   second product as two terms of the cache's 16-bit type (fp16 for e4m3): 16 to
+   17 bits with a bf16 cache, 22 with the others, so that the rounding of the
+   result is what shows; sums and maxima are fp32.  Capped scores are exact to
+   2^-21 of themselves for any cap (beyond 2^-100 .. 2^100: as at those).
    q_out / q_scales (optional, bf16 out, head_dim a multiple of 128): the
    result also as e4m3 [batch, heads * head_dim] with fp32 scales [batch,
    heads * head_dim / 128], the bytes dg_quantize_act makes from `out`.
