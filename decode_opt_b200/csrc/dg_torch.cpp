@@ -380,7 +380,9 @@ PyObject* rotary(PyObject*, PyObject* const* arg, Py_ssize_t count) {
     a.max_position = static_cast<int>(table.size(0));
     a.rot = static_cast<int>(table.size(1));
     a.cos_sin = data<float>(table);
-    for (int i : {0, 1, 7, 14, 15}) no_gradient(arg[i], "rotary");
+    const char* const call =
+        given(arg[5]) ? "rotary_append" : "rotary, but for q and k without out_q and out_k,";
+    for (int i : {0, 1, 7, 14, 15}) no_gradient(arg[i], call);
     const int64_t axes = whole(arg[8], "axes");
     need(PyBytes_Check(arg[9]) && PyBytes_GET_SIZE(arg[9]) == static_cast<Py_ssize_t>(sizeof(a.axis_of)),
          "words must be the packed axes");
